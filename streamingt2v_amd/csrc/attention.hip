@@ -144,8 +144,8 @@ __global__ __launch_bounds__(NW * 64, 4) void attn_spatial_d64_kernel(
         // 1 in every lane; the wave-uniform test skips the 32 accumulator multiplies of the tile
         const bool rescale = __builtin_amdgcn_ballot_w64(m_new != m_run) != 0;
         m_run = m_new;
-        // packed fp32 math (v_pk_fma_f32 / v_pk_add_f32): the softmax is VALU-bound (32 exp2 + ~110 other VALU ops per tile
-        // against 16 MFMAs), so two scores per instruction where the ISA has it
+        // the softmax is VALU-bound (32 exp2 + ~110 other VALU ops per tile against 16 MFMAs); written on pairs (the build forbids the packed fp32
+        // instructions, which measured the same here)
         uint32_t pk[2][8];
 #ifdef SVD_ATTN_SCALAR_SOFTMAX   /* A/B build (profiles/r02_attn_packed_vs_scalar.txt: +1 % = noise): single-issue fp32 ops instead of the packed forms */
         const float mneg = -m_new;

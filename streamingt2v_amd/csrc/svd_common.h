@@ -35,9 +35,10 @@ __device__ __forceinline__ float gelu_erf_f(float x) {
 
 // The same function on a PAIR (round 4; the GEGLU epilogue of the ff1 GEMMs evaluates 64 of them per lane and output tile and is bound by this VALU
 // work -- SQ counters: VALU pipes active 37 % of the kernel at K = 320 against 33 % MFMA-busy).  Same arithmetic, bit for bit; different instructions:
-// the degree-6 polynomial runs on v_pk_fma_f32 (two elements per issue slot) instead of six v_fmaak_f32 per element, and min(|x|, 7) / max(x, 0) are
+// the degree-6 polynomial is written on pairs (the build forbids the packed fp32 instructions, so it compiles to plain v_fma_f32; a v_pk_fma_f32 costs what two of
+// them cost: the whole job measures 2.398 frames/s without and 2.386 with the packed forms on one card), and min(|x|, 7) / max(x, 0) are
 // single instructions (inline asm: the compiler brackets fminf / fmaxf with a canonicalising v_max x, x in IEEE mode -- three more VALU per element).
-// Round-3 ISA: ~17 instructions per element; this form: ~10.5 (a v_pk_fma_f32 costs what two v_fma_f32 cost: the gain is the five plain ones).
+// Round-3 ISA: ~17 instructions per element; this form saves the five plain ones.
 typedef float svd_f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ svd_f32x2 gelu_erf_f2(svd_f32x2 x) {
     svd_f32x2 t, mx, ax;
