@@ -29,7 +29,7 @@ typedef uint16_t svd_bf16;       /* raw 16-bit element (bf16 or fp16 bits, see `
 /* element type of every 16-bit tensor of a call: fp16 -- the reference's own autocast precision (config.yaml:8 "16-mixed"), the host package's
  * default (ops.DEFAULT_ELEM) and the type every parity bound and bench line is stated in -- or bf16 (what north_star names; same MFMA rate, 8x
  * coarser rounding; selectable, ops.set_element_dtype).  Storage 16 bit, accumulation / statistics fp32 in both.  SVD_DTYPE_F32 only where stated. */
-enum { SVD_DTYPE_BF16 = 0, SVD_DTYPE_F16 = 1, SVD_DTYPE_F32 = 2 };
+enum { SVD_DTYPE_BF16 = 0, SVD_DTYPE_F16 = 1, SVD_DTYPE_F32 = 2, SVD_DTYPE_F8 = 3 /* e4m3 (finite, no infinities), operands of svd_linear_act only */ };
 /* OR-ed into the 16-bit `dtype` of the READERS of the fp32 residual stream (svd_groupnorm_stats / _sums / _apply, svd_layernorm,
  * svd_add_rows): the input X (and svd_layernorm's Xsum / svd_add_rows' Y, which continue the stream) is fp32 with leading dimensions in
  * fp32 elements; the normalised output Y -- a GEMM operand -- stays in the 16-bit type.  The stream option keeps the tensors the
@@ -382,6 +382,46 @@ int svd_vfi_merge(const float* warped0, const float* warped1, const float* mask,
 /* fast-TTA average (Trainer.py:90-94): out = (pred2[0] + rot180(pred2[1])) / 2 on [2][h][w][3] fp32; out_u8 (optional) =
  * (uint8)(out * 255.0f), the truncation of i2v_enhance_interface.py:46-47. */
 int svd_vfi_tta_average(const float* pred2, float* out, uint8_t* out_u8, int32_t h, int32_t w, svd_stream_t stream);
+
+/* ---- pre-norm block with differential attention (ABI v12) ------------------------------------------------------
+ * RMS norm, optionally of a residual sum:  s = x + r;  y = s * gamma / sqrt(mean(s^2) + eps).   csrc/rmsnorm.hip
+ *   X [rows][ldx]  16-bit `dtype`, or fp32 with SVD_RMS_X_F32.     R [rows][ldr] or NULL: 16-bit, or fp32 with SVD_RMS_R_F32.
+ *   S [rows][lds] or NULL: the sum s, in R's type (needs R; S == R with lds == ldr updates the residual stream in place).
+ *   Y [rows][ldy]  16-bit `dtype`; with SVD_RMS_OUT_F8 e4m3 values and yscale[rows] fp32: y = yscale[row] * Y[row], yscale = max |y| / 448 (0 for a row of
+ *     zeros; NaN, with NaN values, for a row whose square sum is not finite in fp32).
+ *   gamma [channels] fp32 or NULL (1).  Any channels >= 1, any alignment and leading dimension of whole elements.  rows == 0 returns SVD_OK. */
+enum { SVD_RMS_X_F32 = 1, SVD_RMS_R_F32 = 2, SVD_RMS_OUT_F8 = 4 };
+int svd_rmsnorm(const void* X, int64_t ldx, const void* R, int64_t ldr, const float* gamma, float eps, void* Y, int64_t ldy, float* yscale,
+                void* S, int64_t lds, int64_t rows, int32_t channels, int32_t flags, int32_t dtype, svd_stream_t stream);
+
+/* Product with bias, activation and residual:  Y[m][n] = act( xscale[m] wscale[n] sum_k X[m][k] W[n][k] + bias[n] ) + R[m][n].   csrc/linear.hip
+ *   X [M][ldx], W [N][ldw] row-major: both of in_dtype -- SVD_DTYPE_F16 | BF16 (== dtype), or SVD_DTYPE_F8 (e4m3, with optional row scales).
+ *   bias [N] fp32 or NULL.  R [M][ldr] or NULL: 16-bit `dtype`, or fp32 with SVD_LIN_RES_F32 (R == Y with equal types and strides adds in place).
+ *   Y [M][ldy]: 16-bit `dtype`, or fp32 with SVD_LIN_OUT_F32.  Y must not overlap X or W.
+ *   Any M, N, K >= 1 (M == 0 returns SVD_OK), any alignment and leading dimensions; X and W rows that are 16-byte aligned with K * element size a multiple
+ *   of 16 take the fast path.  (svd_gemm adds its residual before its activation; this entry adds it after.) */
+enum { SVD_ACT_NONE = 0, SVD_ACT_RELU = 1, SVD_ACT_GELU = 2 /* erf */, SVD_ACT_GELU_TANH = 3, SVD_ACT_SILU = 4 };
+enum { SVD_LIN_RES_F32 = 1, SVD_LIN_OUT_F32 = 2 };
+int svd_linear_act(const void* X, int64_t ldx, const void* W, int64_t ldw, const float* xscale, const float* wscale, const float* bias,
+                   const void* R, int64_t ldr, void* Y, int64_t ldy, int64_t M, int32_t N, int32_t K, int32_t act, int32_t flags,
+                   int32_t in_dtype, int32_t dtype, svd_stream_t stream);
+
+/* Differential attention:  O = (softmax(q1 k1^T / 8) - lambda softmax(q2 k2^T / 8)) V per head,  lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + lambda_init;
+ * with gamma, O <- O * gamma * (1 - lambda_init) / sqrt(mean(O^2) + eps) over the head's 128 channels.   csrc/attn_diff.hip
+ *   Q [batch][n_q][heads][128] (q1 | q2), K [batch][n_k][kv_heads][128] (k1 | k2), V [batch][n_k][kv_heads][128], O like Q: 16-bit `dtype`, strides in
+ *   elements per sequence (_sb), token (_st) and head (_sh), all multiples of 8, pointers 16-byte aligned.  heads % kv_heads == 0: head i reads key / value head
+ *   i / (heads / kv_heads).
+ *   lam [4][64] fp32: lq1, lk1, lq2, lk2.   gamma [128] fp32 or NULL (then eps is not used and nothing is scaled by 1 - lambda_init).
+ *   k_len [batch] or NULL: keys of each sequence (clamped to 0..n_k; NULL: n_k); rows of K and V behind them are not read.
+ *   causal: query i stands at position q_start[b] + i (q_start NULL: the last query stands at the last key) and sees keys up to and including its position.
+ *   A query that sees no key gives zeros; values at positions that it does not see never reach it, NaN and Inf included.
+ *   ws: svd_attn_diff_ws_bytes(...) bytes of scratch memory (16-byte aligned; may be NULL when that is 0), free again when the call's work on `stream` ends. */
+int64_t svd_attn_diff_ws_bytes(int32_t batch, int32_t n_q, int32_t n_k, int32_t heads, int32_t kv_heads);
+int svd_attn_diff(const svd_bf16* Q, int64_t q_sb, int64_t q_st, int64_t q_sh, const svd_bf16* K, int64_t k_sb, int64_t k_st, int64_t k_sh,
+                  const svd_bf16* V, int64_t v_sb, int64_t v_st, int64_t v_sh, svd_bf16* O, int64_t o_sb, int64_t o_st, int64_t o_sh,
+                  const float* lam, float lambda_init, const float* gamma, float eps, const int32_t* k_len, const int32_t* q_start,
+                  int32_t batch, int32_t n_q, int32_t n_k, int32_t heads, int32_t kv_heads, int32_t causal, void* ws, int64_t ws_bytes,
+                  int32_t dtype, svd_stream_t stream);
 
 #ifdef __cplusplus
 }

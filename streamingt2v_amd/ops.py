@@ -923,3 +923,150 @@ def vfi_tta_average(pred2, h, w, want_uint8=False):
     u8 = torch.empty((h, w, 3), dtype=torch.uint8, device=pred2.device) if want_uint8 else None
     check(_lib.svd_vfi_tta_average(_p(pred2), _p(out), _p(u8), h, w, _stream()), "svd_vfi_tta_average")
     return out, u8
+
+
+# ---- pre-norm block with differential attention: norm (8-bit rows) -> product -> attention -> product + residual ----
+F8 = torch.float8_e4m3fn
+_SIXTEEN = (BF16, F16)
+
+
+def _ld(t):
+    """Row stride of a 2-D tensor whose columns are contiguous (a single row has no stride to speak of)."""
+    rows, cols = t.shape
+    assert cols <= 1 or t.stride(1) == 1, "rows need contiguous columns"
+    return t.stride(0) if rows > 1 else cols
+
+
+def _on(x, *others):
+    """Every tensor on x's GPU."""
+    assert x.is_cuda and all(t is None or t.device == x.device for t in others), "all tensors must be on one GPU"
+    return x.device
+
+
+def _vec(t, n):
+    """Is t absent or a contiguous fp32 vector of n values?"""
+    return t is None or (t.dtype == torch.float32 and t.shape == (n,) and (n == 1 or t.stride(0) == 1))
+
+
+def rmsnorm(x, gamma=None, *, eps=1e-6, residual=None, f8=False, out=None, out_sum=None):
+    """s = x (+ residual); y = s * gamma / sqrt(mean(s^2) + eps) per row.
+
+    x [rows, C]: 16-bit, or fp32 (the result is then in ops.ELEM); residual [rows, C] of x's 16-bit type (ops.ELEM's for an fp32 x) or fp32; gamma [C] fp32 or None.
+    Returns y (16-bit); with f8=True the pair (q e4m3, scale [rows] fp32), y = scale[row] * q[row]; with a residual the sum s, in the residual's type, follows.
+    out / out_sum: destinations with contiguous columns; out_sum may be the residual itself (the stream goes on in place)."""
+    dev = _on(x, gamma, residual, out, out_sum)
+    assert x.dim() == 2 and (x.dtype in _SIXTEEN or x.dtype == torch.float32)
+    rows, Cc = x.shape
+    e = ELEM if x.dtype == torch.float32 else x.dtype
+    assert _vec(gamma, Cc)
+    assert residual is None or (residual.shape == x.shape and residual.dtype in (e, torch.float32))
+    assert out_sum is None or (residual is not None and out_sum.shape == x.shape and out_sum.dtype == residual.dtype)
+    assert out is None or (out.shape == x.shape and out.dtype == (F8 if f8 else e))
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return rmsnorm(x, gamma, eps=eps, residual=residual, f8=f8, out=out, out_sum=out_sum)
+    y = out if out is not None else torch.empty((rows, Cc), dtype=F8 if f8 else e, device=dev)
+    flags, scale, s, r_ptr, ldr, s_ptr, lds = 0, None, None, None, 0, None, 0
+    if x.dtype == torch.float32:
+        flags |= _l.RMS_X_F32
+    if residual is not None:
+        s = out_sum if out_sum is not None else torch.empty((rows, Cc), dtype=residual.dtype, device=dev)
+        r_ptr, ldr, s_ptr, lds = residual.data_ptr(), _ld(residual), s.data_ptr(), _ld(s)
+        if residual.dtype == torch.float32:
+            flags |= _l.RMS_R_F32
+    if f8:
+        flags |= _l.RMS_OUT_F8
+        scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    if worklog is not None:
+        _wl("rmsnorm", 6.0 * rows * Cc, float(rows) * Cc * (x.element_size() + y.element_size() + (2 * s.element_size() if s is not None else 0)))
+    if rows:
+        check(_lib.svd_rmsnorm(x.data_ptr(), _ld(x), r_ptr, ldr, gamma.data_ptr() if gamma is not None else None, eps, y.data_ptr(), _ld(y),
+                               scale.data_ptr() if f8 else None, s_ptr, lds, rows, Cc, flags, _DT[e], torch.cuda.current_stream().cuda_stream), "svd_rmsnorm")
+    if f8:
+        return (y, scale) if s is None else (y, scale, s)
+    return y if s is None else (y, s)
+
+
+def linear_act(x, w, *, bias=None, act=None, residual=None, x_scale=None, w_scale=None, out_dtype=None, out=None):
+    """Y = act(x_scale[m] w_scale[n] (x W^T)[m, n] + bias[n]) + residual[m, n].
+
+    x [M, K], w [N, K]: both fp16, both bf16, or both e4m3 (x_scale [M], w_scale [N] fp32 or None, e.g. from rmsnorm(f8=True)); bias [N] fp32;
+    act: None | "relu" | "gelu" (erf) | "gelu_tanh" | "silu"; residual [M, N] of the 16-bit type or fp32, added AFTER the activation.
+    The result is of out_dtype: the 16-bit type (for e4m3 operands: ops.ELEM, or the one named) or fp32.  out: a destination with contiguous columns; it may be
+    the residual itself."""
+    dev = _on(x, w, bias, residual, x_scale, w_scale, out)
+    assert x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1] and x.dtype == w.dtype and act in _l.ACT
+    M, K = x.shape
+    N = w.shape[0]
+    f8 = x.dtype == F8
+    assert f8 or x.dtype in _SIXTEEN
+    assert f8 or (x_scale is None and w_scale is None), "row scales belong to 8-bit operands"
+    assert N >= 1 and K >= 1
+    if out_dtype is None:
+        out_dtype = out.dtype if out is not None else (ELEM if f8 else x.dtype)
+    assert out_dtype in _SIXTEEN or out_dtype == torch.float32
+    e = x.dtype
+    if f8:          # the 16-bit type of this call: the output's, else the residual's, else the package's
+        e = out_dtype if out_dtype in _SIXTEEN else residual.dtype if residual is not None and residual.dtype in _SIXTEEN else ELEM
+    assert out_dtype in (e, torch.float32)
+    assert _vec(bias, N) and _vec(x_scale, M) and _vec(w_scale, N)
+    assert residual is None or (residual.shape == (M, N) and residual.dtype in (e, torch.float32))
+    assert out is None or (out.shape == (M, N) and out.dtype == out_dtype)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return linear_act(x, w, bias=bias, act=act, residual=residual, x_scale=x_scale, w_scale=w_scale, out_dtype=out_dtype, out=out)
+    y = out if out is not None else torch.empty((M, N), dtype=out_dtype, device=dev)
+    flags = _l.LIN_OUT_F32 if out_dtype == torch.float32 else 0
+    r_ptr, ldr = None, 0
+    if residual is not None:
+        r_ptr, ldr = residual.data_ptr(), _ld(residual)
+        if residual.dtype == torch.float32:
+            flags |= _l.LIN_RES_F32
+    if worklog is not None:
+        _wl("linear_act", 2.0 * M * N * K, float(M + N) * K * x.element_size() + float(M) * N * (y.element_size() + (residual.element_size() if residual is not None else 0)))
+    if M:
+        check(_lib.svd_linear_act(x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), x_scale.data_ptr() if x_scale is not None else None,
+                                  w_scale.data_ptr() if w_scale is not None else None, bias.data_ptr() if bias is not None else None, r_ptr, ldr, y.data_ptr(),
+                                  _ld(y), M, N, K, _l.ACT[act], flags, _l.DTYPE_F8 if f8 else _DT[e], _DT[e], torch.cuda.current_stream().cuda_stream), "svd_linear_act")
+    return y
+
+
+def _strides4(t):
+    """(sequence, token, head) strides of [batch, n, heads, 128]; a dimension of one has none."""
+    assert t.stride(3) == 1, "a head's 128 channels must be contiguous"
+    return [st if n > 1 else 0 for n, st in zip(t.shape[:3], t.stride()[:3])]
+
+
+def attn_diff(q, k, v, lam, lambda_init, *, gamma=None, eps=1e-5, causal=False, k_len=None, q_start=None, out=None):
+    """Differential attention: (softmax(q1 k1^T / 8) - lambda softmax(q2 k2^T / 8)) v per head, lambda = exp(lq1 . lk1) - exp(lq2 . lk2) + lambda_init; with gamma
+    [128] fp32 followed by an RMS norm over the head's 128 channels, times gamma * (1 - lambda_init).
+
+    q [batch, n_q, heads, 128] (q1 | q2), k [batch, n_k, kv_heads, 128] (k1 | k2), v [batch, n_k, kv_heads, 128]: 16-bit views with 16-byte aligned rows (column
+    ranges of a projection's rows, a cache, (frame, pixel) rows transposed); lam [4, 64] fp32: lq1, lk1, lq2, lk2.
+    k_len [batch] int32: keys of each sequence (rows behind them are not read).  causal: query i of sequence b stands at position q_start[b] + i (int32
+    [batch]; None: the last query stands at the last key) and sees the keys up to there.  A query that sees no key gives zeros.
+    Returns [batch, n_q, heads, 128] (out, if given)."""
+    dev = _on(q, k, v, lam, gamma, k_len, q_start, out)
+    assert q.dim() == 4 and k.dim() == 4 and q.shape[3] == 128 and k.shape == v.shape and k.shape[3] == 128 and k.shape[0] == q.shape[0]
+    assert q.dtype in _SIXTEEN and k.dtype == q.dtype and v.dtype == q.dtype
+    B, n_q, H, _ = q.shape
+    n_k, KV = k.shape[1], k.shape[2]
+    assert KV >= 1 and H >= 1 and H % KV == 0
+    assert lam.dtype == torch.float32 and lam.shape == (4, 64) and lam.is_contiguous()
+    assert _vec(gamma, 128)
+    assert k_len is None or (k_len.dtype == torch.int32 and k_len.shape == (B,) and k_len.is_contiguous())
+    assert q_start is None or (causal and q_start.dtype == torch.int32 and q_start.shape == (B,) and q_start.is_contiguous())
+    assert out is None or (out.shape == q.shape and out.dtype == q.dtype)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return attn_diff(q, k, v, lam, lambda_init, gamma=gamma, eps=eps, causal=causal, k_len=k_len, q_start=q_start, out=out)
+    o = out if out is not None else torch.empty((B, n_q, H, 128), dtype=q.dtype, device=dev)
+    if worklog is not None:
+        _wl("attn_diff", 512.0 * B * H * n_q * n_k, 2.0 * 128 * B * (2 * H * n_q + 2 * KV * n_k))
+    need = _lib.svd_attn_diff_ws_bytes(B, n_q, n_k, H, KV)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None          # from the allocator, per call: its stream and its graph's pool own it
+    check(_lib.svd_attn_diff(q.data_ptr(), *_strides4(q), k.data_ptr(), *_strides4(k), v.data_ptr(), *_strides4(v), o.data_ptr(), *_strides4(o), lam.data_ptr(),
+                             lambda_init, gamma.data_ptr() if gamma is not None else None, eps, k_len.data_ptr() if k_len is not None else None,
+                             q_start.data_ptr() if q_start is not None else None, B, n_q, n_k, H, KV, int(causal), ws.data_ptr() if ws is not None else None,
+                             max(need, 0), _DT[q.dtype], torch.cuda.current_stream().cuda_stream), "svd_attn_diff")
+    return o
