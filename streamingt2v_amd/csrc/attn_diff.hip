@@ -16,6 +16,7 @@
 namespace {
 
 constexpr float LOG2E = 1.44269504088896341f;
+constexpr int PART = 260;                      // floats of one row's share: two accumulators, maximum and sum of each map
 constexpr float M_NONE = -3.0e38f;            // running maximum before the first visible key: finite, so that no -inf - -inf appears
 
 struct DiffArgs {
@@ -44,9 +45,9 @@ __device__ __forceinline__ int seen_by(const DiffArgs& p, int b, int len, int q)
 }
 
 // What a query does not see must not reach it, and a weight of 0 is no help against an Inf or NaN in V: 0 * NaN is NaN.  In a tile that some of the block's
-// queries see further into than others, non-finite values are looked for; if there are any, the products run on V with zeros in their places, and a second product
-// -- of the places with the 0 / 1 mask -- counts for each (channel, query) the non-finite values that it does see: those results become NaN (what p * NaN, and
-// inf - lambda inf, come to).  Rare, so it is a branch of its own.
+// queries see further into than others, non-finite values are looked for; if there are any, the block starts over in a form that multiplies with V with zeros in
+// their places, and counts with a second product -- of the places with the 0 / 1 mask -- the non-finite values that each (channel, query) does see: those
+// results become NaN (what p * NaN, and inf - lambda inf, come to).  Starting over keeps the rare form's registers out of the loop that always runs.
 template <class E> struct NonFinite {
     static constexpr uint32_t EXP = E::kId == SVD_DTYPE_F16 ? 0x7C00u : 0x7F80u, ONE = E::kId == SVD_DTYPE_F16 ? 0x3C00u : 0x3F80u;
     static __device__ __forceinline__ bool any(uint4 w) { return bad(w.x) | bad(w.y) | bad(w.z) | bad(w.w); }
@@ -61,98 +62,130 @@ template <class E> struct NonFinite {
     static __device__ __forceinline__ uint4 cleared(uint4 w) { return make_uint4(cleared(w.x), cleared(w.y), cleared(w.z), cleared(w.w)); }
 };
 
-// One wave per (sequence, key / value head, 32 rows).
-template <class E> __global__ __launch_bounds__(64) void attn_diff_kernel(DiffArgs p, int row_blocks) {
-    __shared__ __attribute__((aligned(16))) uint16_t sV[32][128 + 8];
-    const int lane = threadIdx.x, l31 = lane & 31, hi = lane >> 5;
-    const int rb = blockIdx.x % row_blocks, bh = blockIdx.x / row_blocks, h = bh % p.kv_heads, b = bh / p.kv_heads;
-    const int rows = p.n_q * p.group, row = rb * 32 + l31;
-    const bool live = row < rows;
-    const int q = (live ? row : rows - 1) / p.group, head = h * p.group + (live ? row : rows - 1) % p.group;
-    const int len = key_count(p, b), seen = seen_by(p, b, len, q);
-    const int last = seen_by(p, b, len, min(rows - 1, rb * 32 + 31) / p.group);         // causal or not, the block's last row sees the most keys
-    const int first = p.causal ? seen_by(p, b, len, rb * 32 / p.group) : last;          // ... and its first row the fewest
-    const svd_bf16* Qr = p.Q + b * p.q_sb + q * p.q_st + head * p.q_sh;
-    const svd_bf16* Kb = p.K + b * p.k_sb + h * p.k_sh;
-    const svd_bf16* Vb = p.V + b * p.v_sb + h * p.v_sh;
+// ---- LDS tiles: KT keys of 256 bytes (k1 | k2, or v), 16-byte slots swizzled by the key, written by LDS-DMA (4 rows per instruction, lane = row * 16 + slot) ----
+//   K: slot ^ (key & 15): 16 lanes that read one slot of 16 different keys (ds_read_b128, A operand: lane = key) touch all 64 banks once;
+//   V: slot ^ (4 (key & 3)): a transposing read takes 4 keys x 16 channels per 16 lanes; 32 lanes touch 4 keys x 2 x 32 bytes, all 64 banks once.
+constexpr int ROW_B = 256;
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ void stage_rows(const svd_bf16* base, int64_t stride, int key0, int last, uint32_t dst, int lane, bool v) {
+    const int row = (key0 & 31) + (lane >> 4);                       // key0 is a multiple of 4; the swizzle looks at the low 4 bits of the row in its tile
+    const int slot = (lane & 15) ^ (v ? (row & 3) << 2 : row & 15);
+    const int key = min(key0 + (lane >> 4), last - 1);               // rows behind the last visible key repeat it: they are masked, and hold nothing that is not seen
+    glds16_asm(base + (int64_t)key * stride + slot * 8, dst);
+}
+
+template <class E> struct DiffWave {
     uint4 qf[2][4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int s = 0; s < 4; ++s) qf[i][s] = *(const uint4*)(Qr + 64 * i + 16 * s + 8 * hi);
     f32x16_t o[2][4];
-    float m[2] = {M_NONE, M_NONE}, l[2] = {0.f, 0.f};
+    float m[2], l[2];
+    int l31, hi, seen, first;          // keys that this lane's query sees; the fewest that any query of the wave sees
+    bool bad;                          // a value that is not finite in a tile with hidden places
+    uint32_t ka[8], va[4];             // byte offsets of the lane's K and V^T fragments in a 32-key tile
+
+    __device__ __forceinline__ void init(const svd_bf16* Qr, int lane) {
+        l31 = lane & 31; hi = lane >> 5; bad = false;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+            for (int s = 0; s < 4; ++s) qf[i][s] = *(const uint4*)(Qr + 64 * i + 16 * s + 8 * hi);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[i][t][r] = 0.f;
-    const float c = 0.125f * LOG2E;
-    for (int k0 = 0; k0 < last; k0 += 32) {
-        __syncthreads();
-        for (int e = lane; e < 32 * 16; e += 64) {
-            const int key = k0 + (e >> 4);          // rows behind the last visible key are zeros: nothing of them can reach a product
-            *(uint4*)&sV[e >> 4][(e & 15) * 8] = key < last ? *(const uint4*)(Vb + (int64_t)key * p.v_st + (e & 15) * 8) : make_uint4(0, 0, 0, 0);
-        }
-        __syncthreads();
-        const svd_bf16* Kr = Kb + (int64_t)min(k0 + l31, last - 1) * p.k_st;
-        uint32_t pk[2][8];
+        for (int j = 0; j < 8; ++j) ka[j] = l31 * ROW_B + (((2 * j + hi) ^ (l31 & 15)) << 4);
+        const int i16 = lane & 15, g = (lane >> 4) & 1;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) va[t] = (4 * hi + (i16 >> 2)) * ROW_B + (((4 * t + 2 * g + ((i16 & 3) >> 1)) ^ ((i16 >> 2) << 2)) << 4) + (i16 & 1) * 8;
+    }
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            f32x16_t s;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) s = E::mfma(*(const uint4*)(Kr + 64 * i + 16 * ks + 8 * hi), qf[i][ks], s);
-            float mx = M_NONE;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int key = k0 + 8 * (r >> 2) + 4 * hi + (r & 3);
-                s[r] = key < seen ? s[r] * c : -INFINITY;
-                mx = fmaxf(mx, s[r]);
-            }
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float m_new = fmaxf(m[i], mx), alpha = __builtin_amdgcn_exp2f(m[i] - m_new);
-            m[i] = m_new;
-            float sum = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(s[r] - m_new), p1 = __builtin_amdgcn_exp2f(s[r + 1] - m_new);
-                sum += p0 + p1;
-                pk[i][r >> 1] = E::pack(p0, p1);
-            }
-            l[i] = l[i] * alpha + sum;
+            m[i] = M_NONE; l[i] = 0.f;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[i][t][r] *= alpha;
+                for (int r = 0; r < 16; ++r) o[i][t][r] = 0.f;
         }
-        auto v_frag = [&](int s, int t) {
-            uint32_t w[4];
+    }
+    static __device__ __forceinline__ uint4 k_frag(uint32_t addr) {
+        return __builtin_bit_cast(uint4, *(const __attribute__((address_space(3))) u32x4_t*)addr);
+    }
+    // 8 keys of one channel: 16 s + 4 h + (0..3) and 8 further on
+    static __device__ __forceinline__ uint4 v_frag(uint32_t addr) {
+        typedef __attribute__((address_space(3))) s16x4_t lds_t;
+        const uint2 a = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)addr));
+        const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(addr + 8 * ROW_B)));
+        return make_uint4(a.x, a.y, b.x, b.y);
+    }
+    // 32 keys from k0 on, their K rows at sK and V rows at sV (LDS addresses)
+    template <bool CLEAR> __device__ __forceinline__ void tile(uint32_t sK, uint32_t sV, int k0) {
+        const bool partial = k0 + 32 > first;          // some query of the wave does not see all of the tile
+        const float c = 0.125f * LOG2E;
+        uint32_t pk[2][8];
+        f32x16_t s[2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int key = 16 * s + 8 * (j >> 1) + 4 * hi + 2 * (j & 1);
-                w[j] = sV[key][32 * t + l31] | ((uint32_t)sV[key + 1][32 * t + l31] << 16);
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[i][r] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) s[i] = E::mfma(k_frag(sK + ka[4 * i + ks]), qf[i][ks], s[i]);
+        }
+        if (partial) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const bool hidden = k0 + 8 * (r >> 2) + 4 * hi + (r & 3) >= seen;
+                s[0][r] = hidden ? -INFINITY : s[0][r];
+                s[1][r] = hidden ? -INFINITY : s[1][r];
             }
-            return make_uint4(w[0], w[1], w[2], w[3]);
-        };
-        auto p_frag = [&](int i, int s) { return make_uint4(pk[i][4 * s], pk[i][4 * s + 1], pk[i][4 * s + 2], pk[i][4 * s + 3]); };
-        bool bad = false;
-        if (k0 + 32 > first) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int t = 0; t < 4; ++t) bad |= NonFinite<E>::any(v_frag(s, t));
         }
-        if (__builtin_amdgcn_ballot_w64(bad) == 0) {
+        float mx[2];
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+        for (int i = 0; i < 2; ++i) {
+            mx[i] = fmaxf(s[i][0], s[i][1]);
+#pragma unroll
+            for (int r = 2; r < 16; ++r) mx[i] = fmaxf(mx[i], s[i][r]);
+            mx[i] = fmaxf(mx[i], __shfl_xor(mx[i], 32, 64)) * c;
+        }
+        // The maximum is only there to keep the weights in range: it follows when some query of the wave is 2^8 behind (weights up to 2^8 are as exact as weights up
+        // to 1), not at every new maximum, of which 64 rows have one in almost every tile of the first 2000 keys.  128 multiplications each time.
+        if (__builtin_amdgcn_ballot_w64(mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float m_new = fmaxf(m[i], mx[i]), alpha = __builtin_amdgcn_exp2f(m[i] - m_new);
+                m[i] = m_new;
+                l[i] *= alpha;
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[i][t][r] *= alpha;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i][r], c, -m[i])), p1 = __builtin_amdgcn_exp2f(fmaf(s[i][r + 1], c, -m[i]));
+                sum += p0 + p1;
+                pk[i][r >> 1] = E::pack(p0, p1);
+            }
+            l[i] += sum;
+        }
+        auto p_frag = [&](int i, int q) { return make_uint4(pk[i][4 * q], pk[i][4 * q + 1], pk[i][4 * q + 2], pk[i][4 * q + 3]); };
+        if constexpr (!CLEAR) {
+            if (partial) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) bad |= NonFinite<E>::any(v_frag(sV + va[t] + q * 16 * ROW_B));
+                asm volatile("" ::: "memory");          // the fragments are read again below: 64 registers less
+            }
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    const uint4 vf = v_frag(s, t);
+                    const uint4 vf = v_frag(sV + va[t] + q * 16 * ROW_B);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) o[i][t] = E::mfma(vf, p_frag(i, s), o[i][t]);
+                    for (int i = 0; i < 2; ++i) o[i][t] = E::mfma(vf, p_frag(i, q), o[i][t]);
                 }
         } else {
 #pragma unroll
@@ -161,61 +194,218 @@ template <class E> __global__ __launch_bounds__(64) void attn_diff_kernel(DiffAr
 #pragma unroll
                 for (int r = 0; r < 16; ++r) hit[r] = 0.f;
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const uint4 vf = v_frag(s, t);
+                for (int q = 0; q < 2; ++q) {
+                    const uint4 vf = v_frag(sV + va[t] + q * 16 * ROW_B);
                     uint32_t see[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int key = k0 + 16 * s + 8 * (j >> 1) + 4 * hi + 2 * (j & 1);
+                        const int key = k0 + 16 * q + 8 * (j >> 1) + 4 * hi + 2 * (j & 1);
                         see[j] = (key < seen ? NonFinite<E>::ONE : 0u) | (key + 1 < seen ? NonFinite<E>::ONE << 16 : 0u);
                     }
                     hit = E::mfma(NonFinite<E>::places(vf), make_uint4(see[0], see[1], see[2], see[3]), hit);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) o[i][t] = E::mfma(NonFinite<E>::cleared(vf), p_frag(i, s), o[i][t]);
+                    for (int i = 0; i < 2; ++i) o[i][t] = E::mfma(NonFinite<E>::cleared(vf), p_frag(i, q), o[i][t]);
                 }
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (hit[r] > 0.f) o[0][t][r] = NAN;
+                for (int r = 0; r < 16; ++r) o[0][t][r] = hit[r] > 0.f ? NAN : o[0][t][r];
             }
         }
     }
-    const float lam = diff_lambda(p.lam, p.lambda_init, lane);
-    float w[2];
+    __device__ __forceinline__ void join_halves() {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        l[i] += __shfl_xor(l[i], 32, 64);
-        w[i] = l[i] == 0.f ? 0.f : 1.f / l[i];
+        for (int i = 0; i < 2; ++i) l[i] += __shfl_xor(l[i], 32, 64);
     }
-    w[1] *= lam;
-    float ss = 0.f;
+    // (A_1 - lambda A_2) V, the head's norm, one rounding
+    __device__ __forceinline__ void finish(const DiffArgs& p, svd_bf16* Or, bool live, int lane) {
+        const float lam = diff_lambda(p.lam, p.lambda_init, lane);
+        join_halves();
+        const float w0 = l[0] == 0.f ? 0.f : 1.f / l[0], w1 = l[1] == 0.f ? 0.f : lam / l[1];
+        float ss = 0.f;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            o[0][t][r] = o[0][t][r] * w[0] - o[1][t][r] * w[1];
-            ss = fmaf(o[0][t][r], o[0][t][r], ss);
+            for (int r = 0; r < 16; ++r) {
+                o[0][t][r] = o[0][t][r] * w0 - o[1][t][r] * w1;
+                ss = fmaf(o[0][t][r], o[0][t][r], ss);
+            }
+        ss += __shfl_xor(ss, 32, 64);
+        const float norm = p.gamma ? (1.f - p.lambda_init) / sqrtf(ss * (1.f / 128.f) + p.eps) : 1.f;
+        if (!live) return;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int d = 32 * t + 2 * r + 4 * hi;
+                float y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = o[0][t][r + j] * (p.gamma ? norm * p.gamma[d + j] : 1.f);
+                *(uint2*)(Or + d) = make_uint2(E::pack(y[0], y[1]), E::pack(y[2], y[3]));
+            }
+    }
+};
+
+// Many queries: a workgroup of four waves holds 4 x 32 rows and walks the keys in tiles of 64, staged once for all four, two tiles in turn.
+template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kernel(DiffArgs p, int row_blocks) {
+    constexpr int KT = 64, TILE_B = KT * ROW_B, BUF_B = 2 * TILE_B;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const uint32_t lds = lds_addr_of(smem);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int wg;          // consecutive workgroups go round the 8 XCDs: give each XCD whole heads, whose keys and values stay in its L2
+    {
+        const int n = gridDim.x, x = blockIdx.x & 7, q = n >> 3, r = n & 7;
+        wg = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (blockIdx.x >> 3);
+    }
+    const int rb = row_blocks - 1 - wg % row_blocks, bh = wg / row_blocks, h = bh % p.kv_heads, b = bh / p.kv_heads;      // causal: the longest rows first
+    const int rows = p.n_q * p.group, row0 = rb * 128 + wave * 32, row = row0 + (lane & 31);
+    const bool live = row < rows;
+    const int rc = min(row, rows - 1), q = rc / p.group, head = h * p.group + rc % p.group;
+    const int len = key_count(p, b);
+    const int last = seen_by(p, b, len, min(rows - 1, rb * 128 + 127) / p.group);                 // the workgroup's last row sees the most keys
+    const int mine = row0 < rows ? seen_by(p, b, len, min(rows - 1, row0 + 31) / p.group) : 0;    // ... and the wave's
+    DiffWave<E> w;
+    w.init(p.Q + b * p.q_sb + q * p.q_st + head * p.q_sh, lane);
+    w.seen = seen_by(p, b, len, q);
+    w.first = seen_by(p, b, len, min(rows - 1, row0) / p.group);
+    const svd_bf16* Kb = p.K + b * p.k_sb + h * p.k_sh;
+    const svd_bf16* Vb = p.V + b * p.v_sb + h * p.v_sh;
+    auto stage = [&](int k0, int buf) {          // 16 + 16 KiB by four waves: 4 + 4 instructions each
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = (j * 4 + wave) * 4;
+            const uint32_t dst = __builtin_amdgcn_readfirstlane(lds + buf * BUF_B + r * ROW_B);
+            stage_rows(Kb, p.k_st, k0 + r, last, dst, lane, false);
+            stage_rows(Vb, p.v_st, k0 + r, last, dst + TILE_B, lane, true);
         }
-    ss += __shfl_xor(ss, 32, 64);
-    const float norm = p.gamma ? (1.f - p.lambda_init) / sqrtf(ss * (1.f / 128.f) + p.eps) : 1.f;
+    };
+    auto walk = [&]<bool CLEAR>() {
+        w.clear();
+        if (last > 0) stage(0, 0);
+        int cur = 0;
+        for (int k0 = 0; k0 < last; k0 += KT, cur ^= 1) {
+            svd_wait_dma();
+            __syncthreads();
+            if (k0 + KT < last) stage(k0 + KT, cur ^ 1);
+            const uint32_t sK = lds + cur * BUF_B, sV = sK + TILE_B;
+#pragma unroll 1
+            for (int j = 0; j < KT; j += 32)
+                if (k0 + j < mine) w.template tile<CLEAR>(sK + j * ROW_B, sV + j * ROW_B, k0 + j);
+        }
+    };
+    walk.template operator()<false>();
+    if (__syncthreads_or(w.bad)) walk.template operator()<true>();
+    w.finish(p, p.O + b * p.o_sb + q * p.o_st + head * p.o_sh, live, lane);
+}
+
+// Few queries: one wave per (sequence, key / value head, 32 rows, share of the keys), no workgroup barrier; tiles of 32 keys, two in turn.  With one share
+// the wave finishes the rows; else it leaves maxima, sums and both accumulators in the scratch memory (fp32, [row][share][260]) for the join.
+template <class E> __global__ __launch_bounds__(64, 2) void attn_diff_wave_kernel(DiffArgs p, int row_blocks, int shares, float* ws) {
+    constexpr int KT = 32, TILE_B = KT * ROW_B, BUF_B = 2 * TILE_B;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const uint32_t lds = lds_addr_of(smem);
+    const int lane = threadIdx.x;
+    const int share = blockIdx.x % shares, u = blockIdx.x / shares, rb = u % row_blocks, bh = u / row_blocks, h = bh % p.kv_heads, b = bh / p.kv_heads;
+    const int rows = p.n_q * p.group, row = rb * 32 + (lane & 31);
+    const bool live = row < rows;
+    const int rc = min(row, rows - 1), q = rc / p.group, head = h * p.group + rc % p.group;
+    const int len = key_count(p, b);
+    const int last = seen_by(p, b, len, min(rows - 1, rb * 32 + 31) / p.group);
+    const int per = ((last + 31) / 32 + shares - 1) / shares * 32, begin = share * per, end = min(last, begin + per);      // shares of the keys there are, not of the capacity
+    DiffWave<E> w;
+    w.init(p.Q + b * p.q_sb + q * p.q_st + head * p.q_sh, lane);
+    w.seen = seen_by(p, b, len, q);
+    w.first = seen_by(p, b, len, rb * 32 / p.group);
+    const svd_bf16* Kb = p.K + b * p.k_sb + h * p.k_sh;
+    const svd_bf16* Vb = p.V + b * p.v_sb + h * p.v_sh;
+    auto stage = [&](int k0, int buf) {
+#pragma unroll
+        for (int r = 0; r < 32; r += 4) {
+            const uint32_t dst = lds + buf * BUF_B + r * ROW_B;
+            stage_rows(Kb, p.k_st, k0 + r, last, dst, lane, false);
+            stage_rows(Vb, p.v_st, k0 + r, last, dst + TILE_B, lane, true);
+        }
+    };
+    auto walk = [&]<bool CLEAR>() {
+        w.clear();
+        if (begin < end) stage(begin, 0);
+        int cur = 0;
+        for (int k0 = begin; k0 < end; k0 += KT, cur ^= 1) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // the reads of the tile that is overwritten next are done
+            if (k0 + KT < end) {
+                stage(k0 + KT, cur ^ 1);
+                asm volatile("s_waitcnt vmcnt(16)" ::: "memory");         // all but the 16 just issued: this tile is there
+            } else {
+                svd_wait_dma();
+            }
+            w.template tile<CLEAR>(lds + cur * BUF_B, lds + cur * BUF_B + TILE_B, k0);
+        }
+    };
+    walk.template operator()<false>();
+    if (__builtin_amdgcn_ballot_w64(w.bad)) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        walk.template operator()<true>();
+    }
+    if (shares == 1) {
+        w.finish(p, p.O + b * p.o_sb + q * p.o_st + head * p.o_sh, live, lane);
+        return;
+    }
+    w.join_halves();
     if (!live) return;
-    svd_bf16* Or = p.O + b * p.o_sb + q * p.o_st + head * p.o_sh;
+    float* part = ws + ((int64_t)(bh * rows + row) * shares + share) * PART;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d = 32 * t + 2 * r + 4 * hi;
-            float y[4];
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = o[0][t][r + j] * (p.gamma ? norm * p.gamma[d + j] : 1.f);
-            *(uint2*)(Or + d) = make_uint2(E::pack(y[0], y[1]), E::pack(y[2], y[3]));
-        }
+            for (int r = 0; r < 16; r += 4) *(float4*)(part + 128 * i + 32 * t + 2 * r + 4 * w.hi) = make_float4(w.o[i][t][r], w.o[i][t][r + 1], w.o[i][t][r + 2], w.o[i][t][r + 3]);
+    if (w.hi == 0) *(float4*)(part + 256) = make_float4(w.m[0], w.l[0], w.m[1], w.l[1]);
+}
+
+// One wave per row: lane = two channels.  The shares join in their order, so the result does not depend on which finished first.
+template <class E> __global__ __launch_bounds__(64) void attn_diff_join_kernel(DiffArgs p, int shares, const float* ws) {
+    const int lane = threadIdx.x, rows = p.n_q * p.group, row = blockIdx.x % rows, bh = blockIdx.x / rows, h = bh % p.kv_heads, b = bh / p.kv_heads;
+    const float* part = ws + (int64_t)blockIdx.x * shares * PART;
+    float m[2] = {M_NONE, M_NONE};
+    for (int s = lane; s < shares; s += 64) { m[0] = fmaxf(m[0], part[s * PART + 256]); m[1] = fmaxf(m[1], part[s * PART + 258]); }
+    m[0] = wave_max(m[0]); m[1] = wave_max(m[1]);
+    float l[2] = {0.f, 0.f}, o[2][2] = {};
+    for (int s = 0; s < shares; ++s) {
+        const float4 ml = *(const float4*)(part + s * PART + 256);
+        const float a0 = __builtin_amdgcn_exp2f(ml.x - m[0]), a1 = __builtin_amdgcn_exp2f(ml.z - m[1]);
+        l[0] = fmaf(ml.y, a0, l[0]); l[1] = fmaf(ml.w, a1, l[1]);
+        const float2 x = *(const float2*)(part + s * PART + 2 * lane), y = *(const float2*)(part + s * PART + 128 + 2 * lane);
+        o[0][0] = fmaf(x.x, a0, o[0][0]); o[0][1] = fmaf(x.y, a0, o[0][1]);
+        o[1][0] = fmaf(y.x, a1, o[1][0]); o[1][1] = fmaf(y.y, a1, o[1][1]);
+    }
+    const float lam = diff_lambda(p.lam, p.lambda_init, lane);
+    const float w0 = l[0] == 0.f ? 0.f : 1.f / l[0], w1 = l[1] == 0.f ? 0.f : lam / l[1];
+    float y0 = o[0][0] * w0 - o[1][0] * w1, y1 = o[0][1] * w0 - o[1][1] * w1;
+    if (p.gamma) {
+        const float norm = (1.f - p.lambda_init) / sqrtf(wave_sum(fmaf(y0, y0, y1 * y1)) * (1.f / 128.f) + p.eps);
+        y0 *= norm * p.gamma[2 * lane]; y1 *= norm * p.gamma[2 * lane + 1];
+    }
+    *(uint32_t*)(p.O + b * p.o_sb + (row / p.group) * p.o_st + (h * p.group + row % p.group) * p.o_sh + 2 * lane) = E::pack(y0, y1);
+}
+
+// Which form: see svd_attn_diff
+struct Plan { bool waves; int row_blocks, shares; int64_t ws; };
+Plan plan_for(int64_t batch, int64_t n_q, int64_t n_k, int64_t heads, int64_t kv_heads) {
+    const int64_t rows = n_q * (heads / kv_heads), bh = batch * kv_heads;
+    Plan r = {true, (int)((rows + 31) / 32), 1, 0};
+    if (rows > 64 && (rows + 127) / 128 * bh >= 128) return {false, (int)((rows + 127) / 128), 1, 0};
+    const int64_t units = r.row_blocks * bh;
+    if (units > 0) {
+        int64_t shares = (2048 + units - 1) / units;
+        if (shares > (n_k + 63) / 64) shares = (n_k + 63) / 64;
+        if (shares > 1) { r.shares = (int)shares; r.ws = rows * bh * shares * PART * 4; }
+    }
+    return r;
 }
 
 }  // namespace
 
 extern "C" int64_t svd_attn_diff_ws_bytes(int32_t batch, int32_t n_q, int32_t n_k, int32_t heads, int32_t kv_heads) {
     if (batch < 0 || n_q < 0 || n_k < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads) return SVD_EINVAL;
-    return 0;
+    return plan_for(batch, n_q, n_k, heads, kv_heads).ws;
 }
 
 extern "C" int svd_attn_diff(const svd_bf16* Q, int64_t q_sb, int64_t q_st, int64_t q_sh, const svd_bf16* K, int64_t k_sb, int64_t k_st, int64_t k_sh,
@@ -223,8 +413,9 @@ extern "C" int svd_attn_diff(const svd_bf16* Q, int64_t q_sb, int64_t q_st, int6
                              const float* lam, float lambda_init, const float* gamma, float eps, const int32_t* k_len, const int32_t* q_start,
                              int32_t batch, int32_t n_q, int32_t n_k, int32_t heads, int32_t kv_heads, int32_t causal, void* ws, int64_t ws_bytes,
                              int32_t dtype, svd_stream_t stream) {
-    const int64_t need = svd_attn_diff_ws_bytes(batch, n_q, n_k, heads, kv_heads);
-    if (need < 0 || ws_bytes < need || (need > 0 && !ws)) return SVD_EINVAL;
+    if (batch < 0 || n_q < 0 || n_k < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads) return SVD_EINVAL;
+    const Plan plan = plan_for(batch, n_q, n_k, heads, kv_heads);
+    if (ws_bytes < plan.ws || (plan.ws > 0 && !ws) || ((uintptr_t)ws & 15)) return SVD_EINVAL;
     if (dtype != SVD_DTYPE_BF16 && dtype != SVD_DTYPE_F16) return SVD_EINVAL;
     if (!(eps >= 0.f) || (q_start && !causal)) return SVD_EINVAL;
     if ((q_sb | q_st | q_sh | k_sb | k_st | k_sh | v_sb | v_st | v_sh | o_sb | o_st | o_sh) & 7) return SVD_EINVAL;
@@ -235,10 +426,18 @@ extern "C" int svd_attn_diff(const svd_bf16* Q, int64_t q_sb, int64_t q_st, int6
     if ((int64_t)n_q * group > 0x7fffff00 || n_k > 0x7fffff00) return SVD_EINVAL;
     const DiffArgs p = {Q, q_sb, q_st, q_sh, K, k_sb, k_st, k_sh, V, v_sb, v_st, v_sh, O, o_sb, o_st, o_sh, lam, lambda_init, gamma, eps, k_len, q_start,
                         n_q, n_k, kv_heads, group, causal};
-    const int row_blocks = (n_q * group + 31) / 32;
-    const int64_t grid = (int64_t)row_blocks * batch * kv_heads;
-    if (grid > 0x7fffffff) return SVD_EINVAL;
-    SVD_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((attn_diff_kernel<E>), dim3((unsigned)grid), dim3(64), 0, (hipStream_t)stream, p, row_blocks));
+    const int64_t grid = (int64_t)plan.row_blocks * batch * kv_heads * plan.shares;
+    if (grid > 0x7fffffff || (int64_t)batch * heads * n_q > 0x7fffffff) return SVD_EINVAL;
+    if (!plan.waves) {
+        constexpr int LDS = 4 * 64 * ROW_B;
+        SVD_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((attn_diff_rows_kernel<E>), dim3((unsigned)grid), dim3(256), LDS, (hipStream_t)stream, p, plan.row_blocks));
+    } else {
+        constexpr int LDS = 4 * 32 * ROW_B;
+        SVD_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((attn_diff_wave_kernel<E>), dim3((unsigned)grid), dim3(64), LDS, (hipStream_t)stream, p, plan.row_blocks, plan.shares, (float*)ws));
+        SVD_CHECK_LAUNCH("attn_diff");
+        if (plan.shares > 1)
+            SVD_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((attn_diff_join_kernel<E>), dim3((unsigned)(batch * heads * n_q)), dim3(64), 0, (hipStream_t)stream, p, plan.shares, (const float*)ws));
+    }
     SVD_CHECK_LAUNCH("attn_diff");
     return SVD_OK;
 }
