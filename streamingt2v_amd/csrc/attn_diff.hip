@@ -17,6 +17,7 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr int PART = 260;                      // floats of one row's share: two accumulators, maximum and sum of each map
+constexpr float C_EXP = 0.125f * LOG2E;        // score scale and base 2 in one factor
 constexpr float M_NONE = -3.0e38f;            // running maximum before the first visible key: finite, so that no -inf - -inf appears
 
 struct DiffArgs {
@@ -76,25 +77,37 @@ __device__ __forceinline__ void stage_rows(const svd_bf16* base, int64_t stride,
     glds16_asm(base + (int64_t)key * stride + slot * 8, dst);
 }
 
-template <class E> struct DiffWave {
-    uint4 qf[2][4];
-    f32x16_t o[2][4];
+// maximum over the two halves of the wave, in both
+__device__ __forceinline__ float halves_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
+// Q_LDS: three of map 2's four query fragments wait in the wave's 3 KiB of LDS instead of 12 registers
+template <class E, bool Q_LDS = false> struct DiffWave {
+    uint4 qf[8];
+    uint4* q_lds;
+    f32x16_t o[2][4], s[2];
+    uint32_t pk[2][8];
     float m[2], l[2];
     int l31, hi, seen, first;          // keys that this lane's query sees; the fewest that any query of the wave sees
     bool bad;                          // a value that is not finite in a tile with hidden places
-    uint32_t ka[8], va[4];             // byte offsets of the lane's K and V^T fragments in a 32-key tile
+    uint32_t ka, va;                   // byte offsets of the lane's first K and V^T fragment in a 32-key tile; the others differ in bits 5..7 (K) and 6, 7 (V)
 
-    __device__ __forceinline__ void init(const svd_bf16* Qr, int lane) {
+    __device__ __forceinline__ void init(const svd_bf16* Qr, int lane, uint4* wave_lds = nullptr) {
+        q_lds = wave_lds + lane;
         l31 = lane & 31; hi = lane >> 5; bad = false;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int s = 0; s < 4; ++s) qf[i][s] = *(const uint4*)(Qr + 64 * i + 16 * s + 8 * hi);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ka[j] = l31 * ROW_B + (((2 * j + hi) ^ (l31 & 15)) << 4);
+            for (int s = 0; s < 4; ++s) {
+                const uint4 f = *(const uint4*)(Qr + 64 * i + 16 * s + 8 * hi);
+                if (Q_LDS && i == 1 && s < 3) q_lds[s * 64] = f;
+                else qf[4 * i + s] = f;
+            }
+        ka = l31 * ROW_B + ((hi ^ (l31 & 15)) << 4);
         const int i16 = lane & 15, g = (lane >> 4) & 1;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) va[t] = (4 * hi + (i16 >> 2)) * ROW_B + (((4 * t + 2 * g + ((i16 & 3) >> 1)) ^ ((i16 >> 2) << 2)) << 4) + (i16 & 1) * 8;
+        va = (4 * hi + (i16 >> 2)) * ROW_B + (((2 * g + ((i16 & 3) >> 1)) ^ ((i16 >> 2) << 2)) << 4) + (i16 & 1) * 8;
     }
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -116,74 +129,75 @@ template <class E> struct DiffWave {
         const uint2 b = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(addr + 8 * ROW_B)));
         return make_uint4(a.x, a.y, b.x, b.y);
     }
-    // 32 keys from k0 on, their K rows at sK and V rows at sV (LDS addresses)
+    __device__ __forceinline__ uint4 q_frag(int i, int ks) const {
+        return Q_LDS && i == 1 && ks < 3 ? q_lds[ks * 64] : qf[4 * i + ks];
+    }
+    // ---- the parts of a step of 32 keys, per map ----
+    // S_i^T = K_i Q_i^T, K rows at LDS address sK
+    __device__ __forceinline__ void scores(int i, uint32_t sK) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[i][r] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) s[i] = E::mfma(k_frag((sK + ka) ^ ((4 * i + ks) << 5)), q_frag(i, ks), s[i]);
+    }
+    __device__ __forceinline__ void hide(int i, int k0) {
+        asm volatile("");          // a branch, not 16 selections in every step
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[i][r] = k0 + 8 * (r >> 2) + 4 * hi + (r & 3) >= seen ? -INFINITY : s[i][r];
+    }
+    __device__ __forceinline__ float top(int i) {          // the query's largest score of the step, times c
+        float mx = fmaxf(s[i][0], s[i][1]);
+#pragma unroll
+        for (int r = 2; r < 16; ++r) mx = fmaxf(mx, s[i][r]);
+        return halves_max(mx) * C_EXP;
+    }
+    // The maximum is only there to keep the weights in range: it follows when some query of the wave is 2^8 behind (weights up to 2^8 are as exact as weights up
+    // to 1), not at every new maximum, of which 64 rows have one in almost every tile of the first 2000 keys.  64 multiplications each time.
+    __device__ __forceinline__ void follow(int i, float mx) {
+        if (__builtin_expect_with_probability(__builtin_amdgcn_ballot_w64(mx > m[i] + 8.f) != 0, 0, 0.999)) {
+            const float m_new = fmaxf(m[i], mx), alpha = __builtin_amdgcn_exp2f(m[i] - m_new);
+            m[i] = m_new;
+            l[i] *= alpha;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[i][t][r] *= alpha;
+        }
+    }
+    // weights of scores 2 e and 2 e + 1
+    __device__ __forceinline__ void weigh(int i, int e) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i][2 * e], C_EXP, -m[i])), p1 = __builtin_amdgcn_exp2f(fmaf(s[i][2 * e + 1], C_EXP, -m[i]));
+        l[i] += p0 + p1;
+        pk[i][e] = E::pack(p0, p1);
+    }
+    __device__ __forceinline__ uint4 p_frag(int i, int q) const { return make_uint4(pk[i][4 * q], pk[i][4 * q + 1], pk[i][4 * q + 2], pk[i][4 * q + 3]); }
+    __device__ __forceinline__ void values(int i, int q, int t, uint32_t sV) { o[i][t] = E::mfma(v_frag(((sV + va) ^ (t << 6)) + q * 16 * ROW_B), p_frag(i, q), o[i][t]); }
+    __device__ __forceinline__ void look_for_bad(uint32_t sV) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) bad |= NonFinite<E>::any(v_frag(((sV + va) ^ (t << 6)) + q * 16 * ROW_B));
+        asm volatile("" ::: "memory");          // the fragments are read again for the products: 64 registers less
+    }
+    // a step of 32 keys from k0 on as one piece
     template <bool CLEAR> __device__ __forceinline__ void tile(uint32_t sK, uint32_t sV, int k0) {
         const bool partial = k0 + 32 > first;          // some query of the wave does not see all of the tile
-        const float c = 0.125f * LOG2E;
-        uint32_t pk[2][8];
-        f32x16_t s[2];
+        scores(0, sK);
+        scores(1, sK);
+        if (partial) { hide(0, k0); hide(1, k0); }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+            follow(i, top(i));
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[i][r] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) s[i] = E::mfma(k_frag(sK + ka[4 * i + ks]), qf[i][ks], s[i]);
+            for (int e = 0; e < 8; ++e) weigh(i, e);
         }
-        if (partial) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const bool hidden = k0 + 8 * (r >> 2) + 4 * hi + (r & 3) >= seen;
-                s[0][r] = hidden ? -INFINITY : s[0][r];
-                s[1][r] = hidden ? -INFINITY : s[1][r];
-            }
-        }
-        float mx[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            mx[i] = fmaxf(s[i][0], s[i][1]);
-#pragma unroll
-            for (int r = 2; r < 16; ++r) mx[i] = fmaxf(mx[i], s[i][r]);
-            mx[i] = fmaxf(mx[i], __shfl_xor(mx[i], 32, 64)) * c;
-        }
-        // The maximum is only there to keep the weights in range: it follows when some query of the wave is 2^8 behind (weights up to 2^8 are as exact as weights up
-        // to 1), not at every new maximum, of which 64 rows have one in almost every tile of the first 2000 keys.  128 multiplications each time.
-        if (__builtin_amdgcn_ballot_w64(mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float m_new = fmaxf(m[i], mx[i]), alpha = __builtin_amdgcn_exp2f(m[i] - m_new);
-                m[i] = m_new;
-                l[i] *= alpha;
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[i][t][r] *= alpha;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float sum = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i][r], c, -m[i])), p1 = __builtin_amdgcn_exp2f(fmaf(s[i][r + 1], c, -m[i]));
-                sum += p0 + p1;
-                pk[i][r >> 1] = E::pack(p0, p1);
-            }
-            l[i] += sum;
-        }
-        auto p_frag = [&](int i, int q) { return make_uint4(pk[i][4 * q], pk[i][4 * q + 1], pk[i][4 * q + 2], pk[i][4 * q + 3]); };
         if constexpr (!CLEAR) {
-            if (partial) {
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) bad |= NonFinite<E>::any(v_frag(sV + va[t] + q * 16 * ROW_B));
-                asm volatile("" ::: "memory");          // the fragments are read again below: 64 registers less
-            }
+            if (partial) look_for_bad(sV);
 #pragma unroll
             for (int q = 0; q < 2; ++q)
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    const uint4 vf = v_frag(sV + va[t] + q * 16 * ROW_B);
+                    const uint4 vf = v_frag(((sV + va) ^ (t << 6)) + q * 16 * ROW_B);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) o[i][t] = E::mfma(vf, p_frag(i, q), o[i][t]);
                 }
@@ -195,7 +209,7 @@ template <class E> struct DiffWave {
                 for (int r = 0; r < 16; ++r) hit[r] = 0.f;
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    const uint4 vf = v_frag(sV + va[t] + q * 16 * ROW_B);
+                    const uint4 vf = v_frag(((sV + va) ^ (t << 6)) + q * 16 * ROW_B);
                     uint32_t see[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -209,6 +223,32 @@ template <class E> struct DiffWave {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[0][t][r] = hit[r] > 0.f ? NAN : o[0][t][r];
             }
+        }
+    }
+    // Half of a step, pipelined: the weights of map i for the step at k0 (its scores are in s[i]) on the vector unit, and at the same time on the matrix unit
+    // the other map's scores from the K rows at sK and its products of weights that are there with the V rows at sV.
+    __device__ __forceinline__ void half(int i, int k0, uint32_t sK, uint32_t sV) {
+        if (__builtin_expect_with_probability(k0 + 32 > first, 0, 0.99)) hide(i, k0);
+        auto vf = [&](int e) { return v_frag(((sV + va) ^ ((e & 3) << 6)) + (e >> 2) * 16 * ROW_B); };
+        auto kf = [&](int ks) { return k_frag((sK + ka) ^ ((4 * (1 - i) + ks) << 5)); };
+        uint4 k[2], x[2], v[4];
+        k[0] = kf(0); x[0] = q_frag(1 - i, 0);
+        v[0] = vf(0); v[1] = vf(1); v[2] = vf(2);
+        follow(i, top(i));
+        // the four score products are a chain on one accumulator: they stand between the products with V, which go round four
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[1 - i][r] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (e + 3 < 8) v[(e + 3) % 4] = vf(e + 3);
+            if (e % 2 == 0) {
+                if (e < 6) { k[(e / 2 + 1) & 1] = kf(e / 2 + 1); x[(e / 2 + 1) & 1] = q_frag(1 - i, e / 2 + 1); }
+                s[1 - i] = E::mfma(k[(e / 2) & 1], x[(e / 2) & 1], s[1 - i]);
+            }
+            o[1 - i][e & 3] = E::mfma(v[e % 4], p_frag(1 - i, e >> 2), o[1 - i][e & 3]);
+            weigh(i, e);
+            asm volatile("" : "+v"(pk[i][e]), "+v"(l[i]));          // made here, not where the next half needs it
+            __builtin_amdgcn_sched_barrier(0);                      // the reads stay where they are: three products (150 cycles) ahead of their use
         }
     }
     __device__ __forceinline__ void join_halves() {
@@ -244,9 +284,13 @@ template <class E> struct DiffWave {
     }
 };
 
-// Many queries: a workgroup of four waves holds 4 x 32 rows and walks the keys in tiles of 64, staged once for all four, two tiles in turn.
+// Many queries: a workgroup of four waves holds 4 x 32 rows and walks the keys in steps of 32, staged once for all four.
+// A step's exponentials keep the vector unit busy for longer (2 x 16 exponentials of 16 cycles and 118 other instructions a lane, 1000 cycles) than its products the
+// matrix unit (24 instructions of 32 cycles), so the two have to run at once inside a wave.  The maps take turns: while map 1's weights of step j are made, the matrix unit
+// does map 2's scores of step j and its products with V of step j - 1; while map 2's weights are made, map 1's scores of step j + 1 and its products with V of step j.
+// So K is read a step ahead and V a step behind: rings of four 8-KiB slots each, requests two steps ahead, one barrier a step.
 template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kernel(DiffArgs p, int row_blocks) {
-    constexpr int KT = 64, TILE_B = KT * ROW_B, BUF_B = 2 * TILE_B;
+    constexpr int SLOT_B = 32 * ROW_B, RING_B = 4 * SLOT_B;          // K ring, then V ring
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const uint32_t lds = lds_addr_of(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -262,37 +306,82 @@ template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kern
     const int len = key_count(p, b);
     const int last = seen_by(p, b, len, min(rows - 1, rb * 128 + 127) / p.group);                 // the workgroup's last row sees the most keys
     const int mine = row0 < rows ? seen_by(p, b, len, min(rows - 1, row0 + 31) / p.group) : 0;    // ... and the wave's
-    DiffWave<E> w;
-    w.init(p.Q + b * p.q_sb + q * p.q_st + head * p.q_sh, lane);
+    DiffWave<E, true> w;
+    w.init(p.Q + b * p.q_sb + q * p.q_st + head * p.q_sh, lane, (uint4*)(smem + 2 * RING_B + wave * 3072));
     w.seen = seen_by(p, b, len, q);
     w.first = seen_by(p, b, len, min(rows - 1, row0) / p.group);
     const svd_bf16* Kb = p.K + b * p.k_sb + h * p.k_sh;
     const svd_bf16* Vb = p.V + b * p.v_sb + h * p.v_sh;
-    auto stage = [&](int k0, int buf) {          // 16 + 16 KiB by four waves: 4 + 4 instructions each
+    // Requests: wave-uniform base in scalars, the lane's offset in 32 bits (32 rows of at most 2^26 bytes).  8 KiB by four waves: two instructions each.
+    const int r0 = wave * 8 + (lane >> 4), c16 = lane & 15;
+    const uint32_t k_row = (uint32_t)p.k_st * 2, v_row = (uint32_t)p.v_st * 2;
+    uint32_t ko[2], vo[2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = (j * 4 + wave) * 4;
-            const uint32_t dst = __builtin_amdgcn_readfirstlane(lds + buf * BUF_B + r * ROW_B);
-            stage_rows(Kb, p.k_st, k0 + r, last, dst, lane, false);
-            stage_rows(Vb, p.v_st, k0 + r, last, dst + TILE_B, lane, true);
+    for (int u = 0; u < 2; ++u) {
+        ko[u] = (r0 + 4 * u) * k_row + ((c16 ^ ((r0 + 4 * u) & 15)) << 4);
+        vo[u] = (r0 + 4 * u) * v_row + ((c16 ^ ((r0 & 3) << 2)) << 4);
+    }
+    auto stage = [&](const svd_bf16* src, uint32_t row_b, const uint32_t* off, int j, uint32_t ring) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            uint32_t o = off[u];
+            if (__builtin_expect_with_probability(j * 32 + 32 > last, 0, 0.99)) {          // rows behind the last visible key repeat it: they are masked, and hold nothing that is not seen
+                const int row = r0 + 4 * u;
+                o -= (row - min(row, last - 1 - j * 32)) * row_b;
+            }
+            glds16_saddr(o, src, __builtin_amdgcn_readfirstlane(ring + (j & 3) * SLOT_B + (wave * 8 + 4 * u) * ROW_B));
         }
     };
-    auto walk = [&]<bool CLEAR>() {
-        w.clear();
-        if (last > 0) stage(0, 0);
-        int cur = 0;
-        for (int k0 = 0; k0 < last; k0 += KT, cur ^= 1) {
-            svd_wait_dma();
-            __syncthreads();
-            if (k0 + KT < last) stage(k0 + KT, cur ^ 1);
-            const uint32_t sK = lds + cur * BUF_B, sV = sK + TILE_B;
+    auto stage_k = [&](int j) { stage(Kb + (int64_t)(j * 32) * p.k_st, k_row, ko, j, lds); };
+    auto stage_v = [&](int j) { stage(Vb + (int64_t)(j * 32) * p.v_st, v_row, vo, j, lds + RING_B); };
+    auto at_k = [&](int j) { return lds + (j & 3) * SLOT_B; };
+    auto at_v = [&](int j) { return lds + RING_B + (j & 3) * SLOT_B; };
+    const int steps = (last + 31) / 32, my_steps = (mine + 31) / 32;
+    w.clear();
+    if (steps > 0) {
+        stage_k(0);
+        if (steps > 1) stage_k(1);
+        stage_v(0);
+        if (steps > 2) { stage_k(2); stage_v(1); }
+        else if (steps > 1) stage_v(1);
+        svd_wait_dma();
+        __syncthreads();
+        w.scores(0, at_k(0));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w.pk[1][e] = 0;                       // no weights of step -1: nothing of V's first rows is added
+        const svd_bf16* kp = Kb + (int64_t)96 * p.k_st;                   // the rows requested next: K of step j + 3, V of step j + 2
+        const svd_bf16* vp = Vb + (int64_t)64 * p.v_st;
 #pragma unroll 1
-            for (int j = 0; j < KT; j += 32)
-                if (k0 + j < mine) w.template tile<CLEAR>(sK + j * ROW_B, sV + j * ROW_B, k0 + j);
+        for (int j = 0; j < steps; ++j) {
+            // K of step j + 1 and V of step j: all but the last request, which is four instructions until the requests run out
+            if (__builtin_expect_with_probability(j + 2 < steps, 1, 0.99)) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+            else svd_wait_dma();
+            __syncthreads();
+            if (j + 3 < steps) stage(kp, k_row, ko, j + 3, lds);           // into the slots that step j - 1 was the last to read
+            if (j + 2 < steps) stage(vp, v_row, vo, j + 2, lds + RING_B);
+            kp += 32 * p.k_st; vp += 32 * p.v_st;
+            if (j < my_steps) {
+                if (__builtin_expect_with_probability(j * 32 + 32 > w.first, 0, 0.99)) w.look_for_bad(at_v(j));
+                w.half(0, j * 32, at_k(j), at_v(j > 0 ? j - 1 : 0));
+                w.half(1, j * 32, at_k(j + 1), at_v(j));
+                if (__builtin_expect_with_probability(j == my_steps - 1, 0, 0.99)) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w.values(1, e >> 2, e & 3, at_v(j));
+                }
+            }
         }
-    };
-    walk.template operator()<false>();
-    if (__syncthreads_or(w.bad)) walk.template operator()<true>();
+        if (__syncthreads_or(w.bad)) {          // once more, one step at a time, without what is not finite
+            w.clear();
+            for (int j = 0; j < steps; ++j) {
+                stage_k(j);
+                stage_v(j);
+                svd_wait_dma();
+                __syncthreads();
+                if (j < my_steps) w.template tile<true>(at_k(j), at_v(j), j * 32);
+                __syncthreads();
+            }
+        }
+    }
     w.finish(p, p.O + b * p.o_sb + q * p.o_st + head * p.o_sh, live, lane);
 }
 
@@ -422,6 +511,7 @@ extern "C" int svd_attn_diff(const svd_bf16* Q, int64_t q_sb, int64_t q_st, int6
     if (batch == 0 || n_q == 0) return SVD_OK;
     if (!Q || !O || !lam || (n_k > 0 && (!K || !V))) return SVD_EINVAL;
     if (((uintptr_t)Q | (uintptr_t)K | (uintptr_t)V | (uintptr_t)O) & 15 || ((uintptr_t)lam | (uintptr_t)gamma | (uintptr_t)k_len | (uintptr_t)q_start) & 3) return SVD_EINVAL;
+    if (k_st < 0 || v_st < 0 || k_st > (1 << 25) || v_st > (1 << 25)) return SVD_EINVAL;          // a tile's rows are addressed with 32-bit offsets
     const int group = heads / kv_heads;
     if ((int64_t)n_q * group > 0x7fffff00 || n_k > 0x7fffff00) return SVD_EINVAL;
     const DiffArgs p = {Q, q_sb, q_st, q_sh, K, k_sb, k_st, k_sh, V, v_sb, v_st, v_sh, O, o_sb, o_st, o_sh, lam, lambda_init, gamma, eps, k_len, q_start,
@@ -429,7 +519,7 @@ extern "C" int svd_attn_diff(const svd_bf16* Q, int64_t q_sb, int64_t q_st, int6
     const int64_t grid = (int64_t)plan.row_blocks * batch * kv_heads * plan.shares;
     if (grid > 0x7fffffff || (int64_t)batch * heads * n_q > 0x7fffffff) return SVD_EINVAL;
     if (!plan.waves) {
-        constexpr int LDS = 4 * 64 * ROW_B;
+        constexpr int LDS = 8 * 32 * ROW_B + 4 * 3072;          // rings and map 2's queries: 76 KiB, two workgroups on a CU (two of 80 do not fit)
         SVD_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((attn_diff_rows_kernel<E>), dim3((unsigned)grid), dim3(256), LDS, (hipStream_t)stream, p, plan.row_blocks));
     } else {
         constexpr int LDS = 4 * 32 * ROW_B;
