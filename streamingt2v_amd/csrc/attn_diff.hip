@@ -70,13 +70,6 @@ constexpr int ROW_B = 256;
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ void stage_rows(const svd_bf16* base, int64_t stride, int key0, int last, uint32_t dst, int lane, bool v) {
-    const int row = (key0 & 31) + (lane >> 4);                       // key0 is a multiple of 4; the swizzle looks at the low 4 bits of the row in its tile
-    const int slot = (lane & 15) ^ (v ? (row & 3) << 2 : row & 15);
-    const int key = min(key0 + (lane >> 4), last - 1);               // rows behind the last visible key repeat it: they are masked, and hold nothing that is not seen
-    glds16_asm(base + (int64_t)key * stride + slot * 8, dst);
-}
-
 // maximum over the two halves of the wave, in both
 __device__ __forceinline__ float halves_max(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
@@ -255,8 +248,9 @@ template <class E, bool Q_LDS = false> struct DiffWave {
 #pragma unroll
         for (int i = 0; i < 2; ++i) l[i] += __shfl_xor(l[i], 32, 64);
     }
-    // (A_1 - lambda A_2) V, the head's norm, one rounding
-    __device__ __forceinline__ void finish(const DiffArgs& p, svd_bf16* Or, bool live, int lane) {
+    // (A_1 - lambda A_2) V, the head's norm, one rounding.  A lane holds 64 channels of one row in pieces of four: the rows go through 8 KiB of the wave's LDS (slots
+    // swizzled by the row) and leave as whole rows, four to an instruction.
+    __device__ __forceinline__ void finish(const DiffArgs& p, int b, int h, int row0, int rows, uint32_t buf, int lane) {
         const float lam = diff_lambda(p.lam, p.lambda_init, lane);
         join_halves();
         const float w0 = l[0] == 0.f ? 0.f : 1.f / l[0], w1 = l[1] == 0.f ? 0.f : lam / l[1];
@@ -270,7 +264,6 @@ template <class E, bool Q_LDS = false> struct DiffWave {
             }
         ss += __shfl_xor(ss, 32, 64);
         const float norm = p.gamma ? (1.f - p.lambda_init) / sqrtf(ss * (1.f / 128.f) + p.eps) : 1.f;
-        if (!live) return;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -279,8 +272,20 @@ template <class E, bool Q_LDS = false> struct DiffWave {
                 float y[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) y[j] = o[0][t][r + j] * (p.gamma ? norm * p.gamma[d + j] : 1.f);
-                *(uint2*)(Or + d) = make_uint2(E::pack(y[0], y[1]), E::pack(y[2], y[3]));
+                typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+                const u32x2_t v = {E::pack(y[0], y[1]), E::pack(y[2], y[3])};
+                *(__attribute__((address_space(3))) u32x2_t*)(buf + l31 * ROW_B + (((d >> 3) ^ (l31 & 15)) << 4) + (d & 4) * 2) = v;
             }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+            const int r = j + (lane >> 4), row = row0 + r;
+            const uint4 v = k_frag(buf + r * ROW_B + (((lane & 15) ^ (r & 15)) << 4));
+            if (row < rows) {
+                const int q = p.group == 1 ? row : row / p.group;
+                *(uint4*)(p.O + b * p.o_sb + q * p.o_st + (h * p.group + row - q * p.group) * p.o_sh + (lane & 15) * 8) = v;
+            }
+        }
     }
 };
 
@@ -300,9 +305,8 @@ template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kern
         wg = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (blockIdx.x >> 3);
     }
     const int rb = row_blocks - 1 - wg % row_blocks, bh = wg / row_blocks, h = bh % p.kv_heads, b = bh / p.kv_heads;      // causal: the longest rows first
-    const int rows = p.n_q * p.group, row0 = rb * 128 + wave * 32, row = row0 + (lane & 31);
-    const bool live = row < rows;
-    const int rc = min(row, rows - 1), q = rc / p.group, head = h * p.group + rc % p.group;
+    const int rows = p.n_q * p.group, row0 = rb * 128 + wave * 32;
+    const int rc = min(row0 + (lane & 31), rows - 1), q = rc / p.group, head = h * p.group + rc % p.group;
     const int len = key_count(p, b);
     const int last = seen_by(p, b, len, min(rows - 1, rb * 128 + 127) / p.group);                 // the workgroup's last row sees the most keys
     const int mine = row0 < rows ? seen_by(p, b, len, min(rows - 1, row0 + 31) / p.group) : 0;    // ... and the wave's
@@ -382,7 +386,7 @@ template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kern
             }
         }
     }
-    w.finish(p, p.O + b * p.o_sb + q * p.o_st + head * p.o_sh, live, lane);
+    w.finish(p, b, h, row0, rows, lds + wave * SLOT_B, lane);
 }
 
 // Few queries: one wave per (sequence, key / value head, 32 rows, share of the keys), no workgroup barrier; tiles of 32 keys, two in turn.  With one share
@@ -405,12 +409,17 @@ template <class E> __global__ __launch_bounds__(64, 2) void attn_diff_wave_kerne
     w.first = seen_by(p, b, len, rb * 32 / p.group);
     const svd_bf16* Kb = p.K + b * p.k_sb + h * p.k_sh;
     const svd_bf16* Vb = p.V + b * p.v_sb + h * p.v_sh;
+    // requests as in the rows kernel; one wave requests all 8 + 8 KiB
+    const int l4 = lane >> 4, c16 = lane & 15;
+    const uint32_t k_row = (uint32_t)p.k_st * 2, v_row = (uint32_t)p.v_st * 2;
     auto stage = [&](int k0, int buf) {
+        const svd_bf16 *ks = Kb + (int64_t)k0 * p.k_st, *vs = Vb + (int64_t)k0 * p.v_st;
+        const int top = min(31, last - 1 - k0);                      // rows behind the last visible key repeat it: they are masked, and hold nothing that is not seen
 #pragma unroll
         for (int r = 0; r < 32; r += 4) {
-            const uint32_t dst = lds + buf * BUF_B + r * ROW_B;
-            stage_rows(Kb, p.k_st, k0 + r, last, dst, lane, false);
-            stage_rows(Vb, p.v_st, k0 + r, last, dst + TILE_B, lane, true);
+            const uint32_t dst = lds + buf * BUF_B + r * ROW_B, row = min(r + l4, top);
+            glds16_saddr(row * k_row + ((c16 ^ l4 ^ (r & 12)) << 4), ks, dst);
+            glds16_saddr(row * v_row + ((c16 ^ (l4 << 2)) << 4), vs, dst + TILE_B);
         }
     };
     auto walk = [&]<bool CLEAR>() {
@@ -434,7 +443,8 @@ template <class E> __global__ __launch_bounds__(64, 2) void attn_diff_wave_kerne
         walk.template operator()<true>();
     }
     if (shares == 1) {
-        w.finish(p, p.O + b * p.o_sb + q * p.o_st + head * p.o_sh, live, lane);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        w.finish(p, b, h, rb * 32, rows, lds, lane);
         return;
     }
     w.join_halves();
@@ -483,7 +493,7 @@ Plan plan_for(int64_t batch, int64_t n_q, int64_t n_k, int64_t heads, int64_t kv
     if (rows > 64 && (rows + 127) / 128 * bh >= 128) return {false, (int)((rows + 127) / 128), 1, 0};
     const int64_t units = r.row_blocks * bh;
     if (units > 0) {
-        int64_t shares = (2048 + units - 1) / units;
+        int64_t shares = (1024 + units - 1) / units;          // four waves on each CU (8 caches of 16-32k keys: 100 us with 640 to 1280 waves, 105 with 2048, 130 with 4096)
         if (shares > (n_k + 63) / 64) shares = (n_k + 63) / 64;
         if (shares > 1) { r.shares = (int)shares; r.ws = rows * bh * shares * PART * 4; }
     }
@@ -522,7 +532,7 @@ extern "C" int svd_attn_diff(const svd_bf16* Q, int64_t q_sb, int64_t q_st, int6
         constexpr int LDS = 8 * 32 * ROW_B + 4 * 3072;          // rings and map 2's queries: 76 KiB, two workgroups on a CU (two of 80 do not fit)
         SVD_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((attn_diff_rows_kernel<E>), dim3((unsigned)grid), dim3(256), LDS, (hipStream_t)stream, p, plan.row_blocks));
     } else {
-        constexpr int LDS = 4 * 32 * ROW_B;
+        const int LDS = (n_k > 32 ? 4 : 2) * 32 * ROW_B;          // one tile needs no second buffer: 8 waves on a CU instead of 5 (25 keys x 23040 heads: 182 us, 300 with two and rows written 8 bytes at a time)
         SVD_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((attn_diff_wave_kernel<E>), dim3((unsigned)grid), dim3(64), LDS, (hipStream_t)stream, p, plan.row_blocks, plan.shares, (float*)ws));
         SVD_CHECK_LAUNCH("attn_diff");
         if (plan.shares > 1)
