@@ -530,7 +530,10 @@ extern "C" int svd_attn_diff(const svd_bf16* Q, int64_t q_sb, int64_t q_st, int6
     if (grid > 0x7fffffff || (int64_t)batch * heads * n_q > 0x7fffffff) return SVD_EINVAL;
     if (!plan.waves) {
         constexpr int LDS = 8 * 32 * ROW_B + 4 * 3072;          // rings and map 2's queries: 76 KiB, two workgroups on a CU (two of 80 do not fit)
-        SVD_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((attn_diff_rows_kernel<E>), dim3((unsigned)grid), dim3(256), LDS, (hipStream_t)stream, p, plan.row_blocks));
+        SVD_DISPATCH_DTYPE(dtype, {
+            SVD_ALLOW_LDS(attn_diff_rows_kernel<E>, LDS);
+            hipLaunchKernelGGL((attn_diff_rows_kernel<E>), dim3((unsigned)grid), dim3(256), LDS, (hipStream_t)stream, p, plan.row_blocks);
+        });
     } else {
         const int LDS = (n_k > 32 ? 4 : 2) * 32 * ROW_B;          // one tile needs no second buffer: 8 waves on a CU instead of 5 (25 keys x 23040 heads: 182 us, 300 with two and rows written 8 bytes at a time)
         SVD_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((attn_diff_wave_kernel<E>), dim3((unsigned)grid), dim3(64), LDS, (hipStream_t)stream, p, plan.row_blocks, plan.shares, (float*)ws));

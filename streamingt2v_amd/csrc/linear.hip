@@ -163,10 +163,285 @@ template <class In, class Eo> __global__ __launch_bounds__(256) void linear_any_
             }
 }
 
+// ---- large products: BM x BN outputs per workgroup of WM x WN waves, each TM x TN tiles of 32 x 32; rows 16-byte aligned ----
+// K goes in steps of 64 bytes through a ring of four LDS slots (rows of 64 bytes, 16-byte chunks swizzled by (row >> 2) & 3: 16 lanes that read one chunk of 16
+// rows touch all 64 banks once), filled by LDS-DMA three steps ahead.  A step multiplies fragments that the step before has read and reads the next step's between its
+// matrix instructions; the one barrier per step only says that a slot may be filled again.
+// W's rows lie in LDS as even, then odd columns of each 64: a lane's two tiles of such a block are two adjacent columns, so results leave (and residuals come) as
+// pairs, 32 lanes a contiguous 128 (fp32: 256) bytes of a row.
+template <int WM_, int WN_, int TM_, int TN_> struct Tile {
+    static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, WAVES = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32, SLOT = (BM + BN) * 64, REQ = (BM + BN) / 16 / WAVES;
+};
+__device__ const uint4 g_zeros = {0, 0, 0, 0};
+
+template <int ACT, int N> __device__ __forceinline__ void act_all(f32x16_t (&acc)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            if constexpr (ACT == SVD_ACT_GELU) {
+                const svd_f32x2 y = gelu_erf_f2(svd_f32x2{acc[i][r], acc[i + 1][r]});
+                acc[i][r] = y[0]; acc[i + 1][r] = y[1];
+            } else {
+                acc[i][r] = act_f(acc[i][r], ACT); acc[i + 1][r] = act_f(acc[i + 1][r], ACT);
+            }
+        }
+}
+
+template <class In, class Eo, class T> __global__ __launch_bounds__(T::WAVES * 64, 2) void linear_tile_kernel(LinArgs p, int tiles_m, int tiles_n) {
+    constexpr int TM = T::TM, TN = T::TN, NF = TM + TN;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const uint32_t lds = lds_addr_of(smem);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
+    // each XCD gets a contiguous piece of the tile list, whose order is 8 tiles of M by all tiles of N: the 32 workgroups of an XCD share 8 bands of X and 4 of W
+    int m0, n0;
+    {
+        const int n = gridDim.x, x = blockIdx.x & 7, q = n >> 3, r = n & 7;
+        const int w = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (blockIdx.x >> 3);
+        const int g = w / (8 * tiles_n), gm = min(8, tiles_m - g * 8), u = w - g * 8 * tiles_n;
+        m0 = (g * 8 + u % gm) * T::BM;
+        n0 = (u / gm) * T::BN;
+    }
+    const int wm = (wave / T::WN) * TM * 32, wn = (wave % T::WN) * TN * 32;
+    // requests: 16 rows of 64 bytes each; a wave's are all of X or all of W
+    constexpr int X_REQ = T::BM / 16;
+    const bool is_x = wave * T::REQ < X_REQ;
+    const char* src = is_x ? p.X + (int64_t)m0 * p.ldx : p.W + (int64_t)n0 * p.ldw;
+    const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
+    uint32_t off[T::REQ];
+#pragma unroll
+    for (int u = 0; u < T::REQ; ++u) {
+        const int r = (wave * T::REQ + u) * 16 + (lane >> 2) - (is_x ? 0 : T::BM);
+        const int n = (r & ~63) | ((r & 31) << 1) | ((r >> 5) & 1);
+        const int row = is_x ? min(r, p.M - 1 - m0) : min(n, p.N - 1 - n0);          // rows behind the last repeat it; their results are not stored
+        off[u] = (uint32_t)row * (uint32_t)(is_x ? p.ldx : p.ldw) + chunk * 16;
+    }
+    const int steps = (p.kbytes + 63) >> 6;
+    auto request = [&](int j) {
+        const uint32_t dst = lds + (j & 3) * T::SLOT + wave * T::REQ * 1024;
+        if (__builtin_expect(j * 64 + 64 <= p.kbytes, 1)) {
+#pragma unroll
+            for (int u = 0; u < T::REQ; ++u) glds16_saddr(off[u], src + j * 64, __builtin_amdgcn_readfirstlane(dst + u * 1024));
+        } else {          // the last step's chunks behind K are zeros
+#pragma unroll
+            for (int u = 0; u < T::REQ; ++u)
+                glds16_asm(j * 64 + chunk * 16 < p.kbytes ? src + j * 64 + off[u] : (const char*)&g_zeros, __builtin_amdgcn_readfirstlane(dst + u * 1024));
+        }
+    };
+    f32x16_t acc[TM * TN];
+#pragma unroll
+    for (int i = 0; i < TM * TN; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+    uint4 f[2][NF][2];
+    const uint32_t la = l31 * 64 + (((2 * hi) ^ ((l31 >> 2) & 3)) << 4);
+    auto read = [&](int j, int set, int e) {          // fragment e: X tiles 0 .. TM - 1, then W tiles
+        const uint32_t at = lds + (j & 3) * T::SLOT + (e < TM ? (wm + 32 * e) * 64 : (T::BM + wn + 32 * (e - TM)) * 64) + la;
+        typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+        f[set][e][0] = __builtin_bit_cast(uint4, *(const __attribute__((address_space(3))) u32x4_t*)at);
+        f[set][e][1] = __builtin_bit_cast(uint4, *(const __attribute__((address_space(3))) u32x4_t*)(at ^ 16));
+    };
+    // the order in which a step's fragments are read for the next: first those that its first products take
+    auto nth = [](int e) { return e == 0 ? 0 : e <= TN ? TM + e - 1 : e - TN; };
+    request(0);
+    if (steps > 1) request(1);
+    if (steps > 2) request(2);
+    svd_wait_dma();
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < NF; ++e) read(0, 0, e);
+    auto step = [&]<int SET>(int j) {
+        if (__builtin_expect(j + 2 < steps, 1)) {          // all but the last request: step j + 1 is there
+            if constexpr (T::REQ == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+            else svd_wait_dma();
+        } else svd_wait_dma();
+        __syncthreads();
+        if (j + 3 < steps) request(j + 3);          // into the slot whose fragments were read in step j - 2
+        constexpr int PASSES = In::kWiden ? 4 : In::kBytes == 1 ? 1 : 2;          // matrix instructions per tile and step
+        int e = 0;
+#pragma unroll
+        for (int h = 0; h < PASSES; ++h)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int n = 0; n < TN; ++n) {
+                    if (e < NF) read(j + 1, SET ^ 1, nth(e));
+                    ++e;
+                    const uint4 *a = f[SET][i], *b = f[SET][TM + n];
+                    f32x16_t& c = acc[i * TN + n];
+                    if constexpr (In::kWiden) {
+                        uint4 x[2], y[2];
+                        Frag<In>::widen(a[h >> 1], x[0], x[1]);
+                        Frag<In>::widen(b[h >> 1], y[0], y[1]);
+                        c = ElemF16::mfma(x[h & 1], y[h & 1], c);
+                    } else if constexpr (In::kBytes == 1) {
+                        Frag<In> x, y;
+                        x.set(a[0], a[1]); y.set(b[0], b[1]);
+                        c = mma64<In>(x, y, c);
+                    } else {
+                        c = In::E::mfma(a[h], b[h], c);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+    };
+    for (int j = 0; j < steps; j += 2) {
+        step.template operator()<0>(j);
+        if (j + 1 < steps) step.template operator()<1>(j + 1);
+    }
+
+    // ---- epilogue ----
+    float* s_xs = (float*)smem;
+    __syncthreads();          // the ring's last reads are done
+    for (int r = tid; r < T::BM; r += T::WAVES * 64) s_xs[r] = p.xs ? p.xs[min(m0 + r, p.M - 1)] : 1.f;
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < TN / 2; ++b) {
+        const int n = n0 + wn + 64 * b + 2 * l31, nc = min(n, p.N - 2);
+        const float w0 = p.ws ? p.ws[nc] : 1.f, w1 = p.ws ? p.ws[nc + 1] : 1.f, b0 = p.bias ? p.bias[nc] : 0.f, b1 = p.bias ? p.bias[nc + 1] : 0.f;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 x4 = *(const float4*)(s_xs + wm + 32 * i + 8 * g + 4 * hi);
+                const float x[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int r = 4 * g + k;
+                    acc[i * TN + 2 * b][r] = fmaf(acc[i * TN + 2 * b][r] * x[k], w0, b0);
+                    acc[i * TN + 2 * b + 1][r] = fmaf(acc[i * TN + 2 * b + 1][r] * x[k], w1, b1);
+                }
+            }
+    }
+    if (p.act == SVD_ACT_RELU) act_all<SVD_ACT_RELU>(acc);
+    else if (p.act == SVD_ACT_GELU) act_all<SVD_ACT_GELU>(acc);
+    else if (p.act == SVD_ACT_GELU_TANH) act_all<SVD_ACT_GELU_TANH>(acc);
+    else if (p.act == SVD_ACT_SILU) act_all<SVD_ACT_SILU>(acc);
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int b = 0; b < TN / 2; ++b) {
+            const int n = n0 + wn + 64 * b + 2 * l31, mb = m0 + wm + 32 * i + 4 * hi;
+            f32x16_t &v0 = acc[i * TN + 2 * b], &v1 = acc[i * TN + 2 * b + 1];
+            if (n >= p.N) continue;
+            if (p.R) {
+#pragma unroll
+              for (int half = 0; half < 16; half += 8) {          // eight rows' residuals in flight
+                float2 res[16];
+#pragma unroll
+                for (int r = half; r < half + 8; ++r) {
+                    const int64_t at = (int64_t)min(mb + 8 * (r >> 2) + (r & 3), p.M - 1) * p.ldr + n;
+                    if (p.res_f32) res[r] = *(const float2*)((const float*)p.R + at);
+                    else { const uint32_t w = *(const uint32_t*)((const uint16_t*)p.R + at); res[r] = make_float2(Eo::lo(w), Eo::hi(w)); }
+                }
+#pragma unroll
+                for (int r = half; r < half + 8; ++r) { v0[r] += res[r].x; v1[r] += res[r].y; }
+              }
+            }
+            auto store = [&](int r) {
+                const int64_t at = (int64_t)(mb + 8 * (r >> 2) + (r & 3)) * p.ldy + n;
+                if (p.out_f32) *(float2*)((float*)p.Y + at) = make_float2(v0[r], v1[r]);
+                else *(uint32_t*)((uint16_t*)p.Y + at) = Eo::pack(v0[r], v1[r]);
+            };
+            if (m0 + T::BM <= p.M) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) store(r);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (mb + 8 * (r >> 2) + (r & 3) < p.M) store(r);
+            }
+        }
+}
+
+// ---- few rows: 32 columns x 32 TM rows per workgroup, its eight waves take 64-byte steps of K in turn and add up through LDS.  No staging: the weights are read
+// once, straight into fragments, and what bounds it is how many of their bytes are in flight; rows of any alignment. ----
+template <class In, class Eo, int TM> __global__ __launch_bounds__(512) void linear_rows_kernel(LinArgs p, int tiles_n) {
+    constexpr int NW = 8;
+    __shared__ __attribute__((aligned(16))) float part[NW][TM * 16][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
+    const int m0 = (blockIdx.x / tiles_n) * 32 * TM, n0 = (blockIdx.x % tiles_n) * 32;
+    const char* wr = p.W + (int64_t)min(n0 + l31, p.N - 1) * p.ldw;
+    const char* xr[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) xr[i] = p.X + (int64_t)min(m0 + 32 * i + l31, p.M - 1) * p.ldx;
+    f32x16_t acc[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
+    constexpr int U = TM == 1 ? 4 : 2;          // steps in flight
+    const int steps = (p.kbytes + 63) >> 6;
+    for (int j0 = wave; j0 < steps; j0 += NW * U) {
+        uint4 w[U][2], x[U][TM][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int kb = (j0 + u * NW) * 64 + 32 * hi;          // behind K: zeros
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                w[u][c] = load_chunk<In::kBytes>(wr, kb + 16 * c, p.kbytes);
+#pragma unroll
+                for (int i = 0; i < TM; ++i) x[u][i][c] = load_chunk<In::kBytes>(xr[i], kb + 16 * c, p.kbytes);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            Frag<In> a, b;
+            b.set(w[u][0], w[u][1]);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                a.set(x[u][i][0], x[u][i][1]);
+                acc[i] = mma64<In>(a, b, acc[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) part[wave][i * 16 + r][lane] = acc[i][r];
+    __syncthreads();
+    for (int o = tid; o < TM * 16 * 64; o += NW * 64) {
+        const int r = o >> 6, ln = o & 63, m = m0 + 32 * (r >> 4) + 8 * ((r & 15) >> 2) + 4 * (ln >> 5) + (r & 3), n = n0 + (ln & 31);
+        if (m >= p.M || n >= p.N) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) v += part[w][r][ln];
+        epilogue<Eo>(p, m, n, v);
+    }
+}
+
+// Which form:
 template <class In, class Eo> int launch(const LinArgs& p, hipStream_t stream) {
-    const int64_t tm = (p.M + 127) / 128, tn = (p.N + 127) / 128;
-    if (tm * tn > 0x7fffffff) return SVD_EINVAL;
-    hipLaunchKernelGGL((linear_any_kernel<In, Eo>), dim3((unsigned)(tm * tn)), dim3(256), 0, stream, p, (int)tn);
+    using Big = Tile<2, 4, 4, 2>;              // 256 x 256, eight waves, 128 KiB: one workgroup on a CU
+    using Small = Tile<2, 2, 2, 2>;            // 128 x 128, four waves, 64 KiB: two
+    auto tiles = [&](int bm, int bn) { return (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+    const uintptr_t pair = p.out_f32 ? (uintptr_t)p.Y & 7 : (uintptr_t)p.Y & 3, rpair = !p.R ? 0 : p.res_f32 ? (uintptr_t)p.R & 7 : (uintptr_t)p.R & 3;
+    const bool aligned = !(((uintptr_t)p.X | (uintptr_t)p.W | p.ldx | p.ldw | p.kbytes) & 15) && !pair && !rpair && !((p.ldy | (p.R ? p.ldr : 0) | p.N) & 1) &&
+                         p.ldx < (1 << 23) && p.ldw < (1 << 23);
+    if (p.M <= 64 || tiles(128, 128) < 64) {
+        const int tm = p.M <= 32 ? 1 : 2;
+        const int64_t tn = (p.N + 31) / 32, grid = (p.M + 32 * tm - 1) / (32 * tm) * tn;
+        if (grid > 0x7fffffff) return SVD_EINVAL;
+        if (tm == 1) hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 1>), dim3((unsigned)grid), dim3(512), 0, stream, p, (int)tn);
+        else hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 2>), dim3((unsigned)grid), dim3(512), 0, stream, p, (int)tn);
+    } else if (!aligned) {
+        const int64_t grid = tiles(128, 128);
+        if (grid > 0x7fffffff) return SVD_EINVAL;
+        hipLaunchKernelGGL((linear_any_kernel<In, Eo>), dim3((unsigned)grid), dim3(256), 0, stream, p, (p.N + 127) / 128);
+    } else {
+        bool big = false;
+        if constexpr (!In::kWiden) {          // (widened fragments do not leave registers for the large tile)
+            big = tiles(256, 256) >= 128;
+            if (big) {
+                if (tiles(256, 256) > 0x7fffffff) return SVD_EINVAL;
+                SVD_ALLOW_LDS((linear_tile_kernel<In, Eo, Big>), 4 * Big::SLOT);
+                hipLaunchKernelGGL((linear_tile_kernel<In, Eo, Big>), dim3((unsigned)tiles(256, 256)), dim3(512), 4 * Big::SLOT, stream, p, (p.M + 255) / 256, (p.N + 255) / 256);
+            }
+        }
+        if (!big) {
+            if (tiles(128, 128) > 0x7fffffff) return SVD_EINVAL;
+            hipLaunchKernelGGL((linear_tile_kernel<In, Eo, Small>), dim3((unsigned)tiles(128, 128)), dim3(256), 4 * Small::SLOT, stream, p, (p.M + 127) / 128, (p.N + 127) / 128);
+        }
+    }
     SVD_CHECK_LAUNCH("linear_act");
     return SVD_OK;
 }

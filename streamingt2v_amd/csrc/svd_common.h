@@ -181,3 +181,15 @@ extern "C" void svd_set_error_(const char* what, hipError_t e);
         hipError_t e__ = hipGetLastError();                     \
         if (e__ != hipSuccess) { svd_set_error_(what, e__); return SVD_ELAUNCH; } \
     } while (0)
+// Lets a kernel have more than 64 KiB of dynamic LDS, once per device (the attribute belongs to the device's copy of the kernel).
+#define SVD_ALLOW_LDS(kernel, bytes)                                                                                                              \
+    do {                                                                                                                                          \
+        static int done__[64] = {0};                                                                                                              \
+        int dev__ = 0;                                                                                                                            \
+        if (hipGetDevice(&dev__) != hipSuccess || dev__ < 0 || dev__ >= 64) return SVD_ELAUNCH;                                                   \
+        if (!__atomic_load_n(&done__[dev__], __ATOMIC_RELAXED)) {                                                                                 \
+            const hipError_t e__ = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);                   \
+            if (e__ != hipSuccess) { svd_set_error_("hipFuncSetAttribute", e__); return SVD_ELAUNCH; }                                            \
+            __atomic_store_n(&done__[dev__], 1, __ATOMIC_RELAXED);                                                                                \
+        }                                                                                                                                         \
+    } while (0)

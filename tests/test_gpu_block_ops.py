@@ -227,10 +227,10 @@ def test_linear_activations_reach_far_values(ops, act, t):
 
 
 @pytest.mark.parametrize("t", [F16, BF16, F8], ids=str)
-@pytest.mark.parametrize("m", [3, 70, 300, 1100])
-def test_linear_picks_rows_and_columns(ops, t, m):
-    """One-hot rows select columns of W: any swapped lane, row or K chunk shows as another number, exactly."""
-    n, k = 272, 208
+@pytest.mark.parametrize("m,n,k", [(3, 272, 208), (70, 272, 208), (300, 272, 208), (1100, 1040, 208), (1100, 1041, 209), (1100, 1040, 80), (4100, 2064, 208), (4100, 2064, 64), (4096, 2048, 320)])
+def test_linear_picks_rows_and_columns(ops, t, m, n, k):
+    """One-hot rows select columns of W: any swapped lane, row or K chunk shows as another number, exactly.  Few rows, 128- and 256-row tiles, unaligned rows, one to
+    many K steps with and without a rest."""
     x = torch.zeros(m, k, device="cuda")
     idx = (torch.arange(m, device="cuda") * 7) % k
     x[torch.arange(m, device="cuda"), idx] = 1
@@ -273,7 +273,7 @@ def test_linear_rows_do_not_mix(ops, t):
 
 @pytest.mark.parametrize("t", [BF16, F8], ids=str)
 def test_linear_product_sizes(ops, t):
-    for i, (m, n, k) in enumerate([(2304, 5120, 1280), (2304, 1280, 5120), (4096, 3840, 1280), (1000, 2560, 640)]):
+    for i, (m, n, k) in enumerate([(2304, 5120, 1280), (2304, 1280, 5120), (4096, 3840, 1280), (1000, 2560, 640), (3000, 2998, 1296), (1111, 1501, 333)]):
         randn, x, w, sx, sw = make_linear(300 + i, m, n, k, t)
         bias, res = randn(n), randn(m, n).to(F32 if i % 2 else BF16)
         got = ops.linear_act(x, w, bias=bias, act="gelu", residual=res, x_scale=sx, w_scale=sw, out_dtype=res.dtype)
