@@ -188,25 +188,105 @@ template <int ACT, int N> __device__ __forceinline__ void act_all(f32x16_t (&acc
         }
 }
 
-template <class In, class Eo, class T> __global__ __launch_bounds__(T::WAVES * 64, 2) void linear_tile_kernel(LinArgs p, int tiles_m, int tiles_n) {
+// TM x TN finished tiles of a wave: scales and bias, activation, residual, one rounding.  m0, n0: the wave's first row and column; xs: its rows' scales (LDS).
+// Columns come and go as pairs; `whole`: all its rows exist.
+template <class Eo, int TM, int TN> __device__ __forceinline__ void finish_tiles(const LinArgs& p, f32x16_t (&acc)[TM * TN], int m0, int n0, const float* xs, bool whole, int l31, int hi) {
+#pragma unroll
+    for (int b = 0; b < TN / 2; ++b) {
+        const int nc = min(n0 + 64 * b + 2 * l31, p.N - 2);
+        const float w0 = p.ws ? p.ws[nc] : 1.f, w1 = p.ws ? p.ws[nc + 1] : 1.f, b0 = p.bias ? p.bias[nc] : 0.f, b1 = p.bias ? p.bias[nc + 1] : 0.f;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 x4 = *(const float4*)(xs + 32 * i + 8 * g + 4 * hi);
+                const float x[4] = {x4.x, x4.y, x4.z, x4.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int r = 4 * g + k;
+                    acc[i * TN + 2 * b][r] = fmaf(acc[i * TN + 2 * b][r] * x[k], w0, b0);
+                    acc[i * TN + 2 * b + 1][r] = fmaf(acc[i * TN + 2 * b + 1][r] * x[k], w1, b1);
+                }
+            }
+    }
+    if (p.act == SVD_ACT_RELU) act_all<SVD_ACT_RELU>(acc);
+    else if (p.act == SVD_ACT_GELU) act_all<SVD_ACT_GELU>(acc);
+    else if (p.act == SVD_ACT_GELU_TANH) act_all<SVD_ACT_GELU_TANH>(acc);
+    else if (p.act == SVD_ACT_SILU) act_all<SVD_ACT_SILU>(acc);
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int b = 0; b < TN / 2; ++b) {
+            const int n = n0 + 64 * b + 2 * l31, mb = m0 + 32 * i + 4 * hi;
+            f32x16_t &v0 = acc[i * TN + 2 * b], &v1 = acc[i * TN + 2 * b + 1];
+            if (n >= p.N) continue;
+            if (p.R) {
+#pragma unroll
+                for (int half = 0; half < 16; half += 8) {          // eight rows' residuals in flight
+                    float2 res[16];
+#pragma unroll
+                    for (int r = half; r < half + 8; ++r) {
+                        const int64_t at = (int64_t)min(mb + 8 * (r >> 2) + (r & 3), p.M - 1) * p.ldr + n;
+                        if (p.res_f32) res[r] = *(const float2*)((const float*)p.R + at);
+                        else { const uint32_t w = *(const uint32_t*)((const uint16_t*)p.R + at); res[r] = make_float2(Eo::lo(w), Eo::hi(w)); }
+                    }
+#pragma unroll
+                    for (int r = half; r < half + 8; ++r) { v0[r] += res[r].x; v1[r] += res[r].y; }
+                }
+            }
+            auto store = [&](int r) {
+                const int64_t at = (int64_t)(mb + 8 * (r >> 2) + (r & 3)) * p.ldy + n;
+                if (p.out_f32) *(float2*)((float*)p.Y + at) = make_float2(v0[r], v1[r]);
+                else *(uint32_t*)((uint16_t*)p.Y + at) = Eo::pack(v0[r], v1[r]);
+            };
+            if (whole) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) store(r);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (mb + 8 * (r >> 2) + (r & 3) < p.M) store(r);
+            }
+        }
+}
+
+// Place of tile `w` of the list: 8 tiles of M by all tiles of N, then the next 8: the 32 workgroups that an XCD runs at once share 8 bands of X and 4 of W.
+__device__ __forceinline__ void tile_place(int w, int tiles_m, int tiles_n, int& tm, int& tn) {
+    const int g = w / (8 * tiles_n), gm = min(8, tiles_m - g * 8), u = w - g * 8 * tiles_n;
+    tm = g * 8 + u % gm;
+    tn = u / gm;
+}
+// Split of a product's last, incomplete round of workgroups: the first `whole` tiles have a workgroup each, the others `shares` of K each, whose sums meet in
+// scratch memory (fp32, [share][wave][tile][4 rows of 4][lane]) and are finished by linear_join_kernel in the order of the shares.
+struct Rounds { int whole, shares; float* ws; };
+
+// SHARE: the launch over the shares of K of the tiles behind the whole ones
+template <class In, class Eo, class T, bool SHARE> __global__ __launch_bounds__(T::WAVES * 64, 2) void linear_tile_kernel(LinArgs p, int tiles_m, int tiles_n, Rounds rd) {
     constexpr int TM = T::TM, TN = T::TN, NF = TM + TN;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const uint32_t lds = lds_addr_of(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
-    // each XCD gets a contiguous piece of the tile list, whose order is 8 tiles of M by all tiles of N: the 32 workgroups of an XCD share 8 bands of X and 4 of W
-    int m0, n0;
+    int m0, n0, k_from = 0, steps = (p.kbytes + 63) >> 6;          // steps of 64 bytes of K
     {
-        const int n = gridDim.x, x = blockIdx.x & 7, q = n >> 3, r = n & 7;
-        const int w = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (blockIdx.x >> 3);
-        const int g = w / (8 * tiles_n), gm = min(8, tiles_m - g * 8), u = w - g * 8 * tiles_n;
-        m0 = (g * 8 + u % gm) * T::BM;
-        n0 = (u / gm) * T::BN;
+        int w;
+        if constexpr (!SHARE) {          // consecutive workgroups go round the 8 XCDs: each gets a contiguous piece of the list
+            const int n = rd.whole, x = blockIdx.x & 7, q = n >> 3, r = n & 7;
+            w = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (blockIdx.x >> 3);
+        } else {
+            w = rd.whole + blockIdx.x / rd.shares;
+            const int share = blockIdx.x % rd.shares, per = (steps + rd.shares - 1) / rd.shares;
+            k_from = min(share * per, steps);
+            steps = min(per, steps - k_from);
+        }
+        tile_place(w, tiles_m, tiles_n, m0, n0);
+        m0 *= T::BM; n0 *= T::BN;
     }
     const int wm = (wave / T::WN) * TM * 32, wn = (wave % T::WN) * TN * 32;
     // requests: 16 rows of 64 bytes each; a wave's are all of X or all of W
     constexpr int X_REQ = T::BM / 16;
     const bool is_x = wave * T::REQ < X_REQ;
-    const char* src = is_x ? p.X + (int64_t)m0 * p.ldx : p.W + (int64_t)n0 * p.ldw;
+    const char* src = (is_x ? p.X + (int64_t)m0 * p.ldx : p.W + (int64_t)n0 * p.ldw) + (int64_t)k_from * 64;
+    const int kbytes = p.kbytes - k_from * 64;
     const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
     uint32_t off[T::REQ];
 #pragma unroll
@@ -216,16 +296,15 @@ template <class In, class Eo, class T> __global__ __launch_bounds__(T::WAVES * 6
         const int row = is_x ? min(r, p.M - 1 - m0) : min(n, p.N - 1 - n0);          // rows behind the last repeat it; their results are not stored
         off[u] = (uint32_t)row * (uint32_t)(is_x ? p.ldx : p.ldw) + chunk * 16;
     }
-    const int steps = (p.kbytes + 63) >> 6;
     auto request = [&](int j) {
         const uint32_t dst = lds + (j & 3) * T::SLOT + wave * T::REQ * 1024;
-        if (__builtin_expect(j * 64 + 64 <= p.kbytes, 1)) {
+        if (__builtin_expect(j * 64 + 64 <= kbytes, 1)) {
 #pragma unroll
             for (int u = 0; u < T::REQ; ++u) glds16_saddr(off[u], src + j * 64, __builtin_amdgcn_readfirstlane(dst + u * 1024));
         } else {          // the last step's chunks behind K are zeros
 #pragma unroll
             for (int u = 0; u < T::REQ; ++u)
-                glds16_asm(j * 64 + chunk * 16 < p.kbytes ? src + j * 64 + off[u] : (const char*)&g_zeros, __builtin_amdgcn_readfirstlane(dst + u * 1024));
+                glds16_asm(j * 64 + chunk * 16 < kbytes ? src + j * 64 + off[u] : (const char*)&g_zeros, __builtin_amdgcn_readfirstlane(dst + u * 1024));
         }
     };
     f32x16_t acc[TM * TN];
@@ -243,7 +322,7 @@ template <class In, class Eo, class T> __global__ __launch_bounds__(T::WAVES * 6
     };
     // the order in which a step's fragments are read for the next: first those that its first products take
     auto nth = [](int e) { return e == 0 ? 0 : e <= TN ? TM + e - 1 : e - TN; };
-    request(0);
+    if (steps > 0) request(0);
     if (steps > 1) request(1);
     if (steps > 2) request(2);
     svd_wait_dma();
@@ -289,68 +368,47 @@ template <class In, class Eo, class T> __global__ __launch_bounds__(T::WAVES * 6
         if (j + 1 < steps) step.template operator()<1>(j + 1);
     }
 
-    // ---- epilogue ----
-    float* s_xs = (float*)smem;
-    __syncthreads();          // the ring's last reads are done
-    for (int r = tid; r < T::BM; r += T::WAVES * 64) s_xs[r] = p.xs ? p.xs[min(m0 + r, p.M - 1)] : 1.f;
-    __syncthreads();
+    if constexpr (SHARE) {          // the sums, as they lie
+        float4* out = (float4*)rd.ws + ((int64_t)blockIdx.x * T::WAVES + wave) * (TM * TN * 4 * 64) + lane;
 #pragma unroll
-    for (int b = 0; b < TN / 2; ++b) {
-        const int n = n0 + wn + 64 * b + 2 * l31, nc = min(n, p.N - 2);
-        const float w0 = p.ws ? p.ws[nc] : 1.f, w1 = p.ws ? p.ws[nc + 1] : 1.f, b0 = p.bias ? p.bias[nc] : 0.f, b1 = p.bias ? p.bias[nc + 1] : 0.f;
+        for (int i = 0; i < TM * TN; ++i)
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+            for (int g = 0; g < 4; ++g) out[(i * 4 + g) * 64] = make_float4(acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]);
+    } else {
+        float* s_xs = (float*)smem;
+        __syncthreads();          // the ring's last reads are done
+        for (int r = tid; r < T::BM; r += T::WAVES * 64) s_xs[r] = p.xs ? p.xs[min(m0 + r, p.M - 1)] : 1.f;
+        __syncthreads();
+        finish_tiles<Eo, TM, TN>(p, acc, m0 + wm, n0 + wn, s_xs + wm, m0 + T::BM <= p.M, l31, hi);
+    }
+}
+
+// One workgroup per split tile and band of 32 rows of its waves: the shares' sums in their order, then the epilogue.
+template <class Eo, class T> __global__ __launch_bounds__(T::WAVES * 64) void linear_join_kernel(LinArgs p, int tiles_m, int tiles_n, Rounds rd) {
+    __shared__ float s_xs[T::WAVES][32];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, t = blockIdx.x / T::TM, i = blockIdx.x % T::TM;
+    int m0, n0;
+    tile_place(rd.whole + t, tiles_m, tiles_n, m0, n0);
+    m0 = m0 * T::BM + (wave / T::WN) * T::TM * 32 + 32 * i;
+    n0 = n0 * T::BN + (wave % T::WN) * T::TN * 32;
+    f32x16_t acc[T::TN];
+#pragma unroll
+    for (int j = 0; j < T::TN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[j][r] = 0.f;
+    for (int s = 0; s < rd.shares; ++s) {
+        const float4* in = (const float4*)rd.ws + ((int64_t)(t * rd.shares + s) * T::WAVES + wave) * (T::TM * T::TN * 4 * 64) + i * T::TN * 4 * 64 + lane;
+#pragma unroll
+        for (int j = 0; j < T::TN; ++j)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const float4 x4 = *(const float4*)(s_xs + wm + 32 * i + 8 * g + 4 * hi);
-                const float x[4] = {x4.x, x4.y, x4.z, x4.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int r = 4 * g + k;
-                    acc[i * TN + 2 * b][r] = fmaf(acc[i * TN + 2 * b][r] * x[k], w0, b0);
-                    acc[i * TN + 2 * b + 1][r] = fmaf(acc[i * TN + 2 * b + 1][r] * x[k], w1, b1);
-                }
+                const float4 v = in[(j * 4 + g) * 64];
+                acc[j][4 * g] += v.x; acc[j][4 * g + 1] += v.y; acc[j][4 * g + 2] += v.z; acc[j][4 * g + 3] += v.w;
             }
     }
-    if (p.act == SVD_ACT_RELU) act_all<SVD_ACT_RELU>(acc);
-    else if (p.act == SVD_ACT_GELU) act_all<SVD_ACT_GELU>(acc);
-    else if (p.act == SVD_ACT_GELU_TANH) act_all<SVD_ACT_GELU_TANH>(acc);
-    else if (p.act == SVD_ACT_SILU) act_all<SVD_ACT_SILU>(acc);
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int b = 0; b < TN / 2; ++b) {
-            const int n = n0 + wn + 64 * b + 2 * l31, mb = m0 + wm + 32 * i + 4 * hi;
-            f32x16_t &v0 = acc[i * TN + 2 * b], &v1 = acc[i * TN + 2 * b + 1];
-            if (n >= p.N) continue;
-            if (p.R) {
-#pragma unroll
-              for (int half = 0; half < 16; half += 8) {          // eight rows' residuals in flight
-                float2 res[16];
-#pragma unroll
-                for (int r = half; r < half + 8; ++r) {
-                    const int64_t at = (int64_t)min(mb + 8 * (r >> 2) + (r & 3), p.M - 1) * p.ldr + n;
-                    if (p.res_f32) res[r] = *(const float2*)((const float*)p.R + at);
-                    else { const uint32_t w = *(const uint32_t*)((const uint16_t*)p.R + at); res[r] = make_float2(Eo::lo(w), Eo::hi(w)); }
-                }
-#pragma unroll
-                for (int r = half; r < half + 8; ++r) { v0[r] += res[r].x; v1[r] += res[r].y; }
-              }
-            }
-            auto store = [&](int r) {
-                const int64_t at = (int64_t)(mb + 8 * (r >> 2) + (r & 3)) * p.ldy + n;
-                if (p.out_f32) *(float2*)((float*)p.Y + at) = make_float2(v0[r], v1[r]);
-                else *(uint32_t*)((uint16_t*)p.Y + at) = Eo::pack(v0[r], v1[r]);
-            };
-            if (m0 + T::BM <= p.M) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) store(r);
-            } else {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (mb + 8 * (r >> 2) + (r & 3) < p.M) store(r);
-            }
-        }
+    if (lane < 32) s_xs[wave][lane] = p.xs ? p.xs[min(m0 + lane, p.M - 1)] : 1.f;
+    __syncthreads();
+    finish_tiles<Eo, 1, T::TN>(p, acc, m0, n0, s_xs[wave], m0 + 32 <= p.M, lane & 31, lane >> 5);
 }
 
 // ---- few rows: 32 columns x 32 TM rows per workgroup, its eight waves take 64-byte steps of K in turn and add up through LDS.  No staging: the weights are read
@@ -409,38 +467,70 @@ template <class In, class Eo, int TM> __global__ __launch_bounds__(512) void lin
     }
 }
 
-// Which form:
-template <class In, class Eo> int launch(const LinArgs& p, hipStream_t stream) {
-    using Big = Tile<2, 4, 4, 2>;              // 256 x 256, eight waves, 128 KiB: one workgroup on a CU
-    using Small = Tile<2, 2, 2, 2>;            // 128 x 128, four waves, 64 KiB: two
-    auto tiles = [&](int bm, int bn) { return (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
+using Big = Tile<2, 4, 4, 2>;              // 256 x 256, eight waves, 128 KiB: one workgroup on a CU
+using Small = Tile<2, 2, 2, 2>;            // 128 x 128, four waves, 64 KiB: two
+constexpr int CUS = 256;
+
+// Which form, from sizes alone.
+enum { ROWS, BIG, SMALL };
+struct LinPlan { int form, whole, shares; int64_t ws; };
+template <class T> LinPlan rounds_of(int form, int64_t tm, int64_t tn, int64_t kbytes, int slots) {
+    const int64_t tiles = tm * tn, rest = tiles % slots, steps = (kbytes + 63) / 64;
+    LinPlan r = {form, (int)tiles, 1, 0};
+    int64_t shares = rest ? slots / rest : 1;
+    if (shares > steps / 8) shares = steps / 8;          // a share of at least 8 steps
+    if (shares > 8) shares = 8;
+    if (shares > 1) { r.whole = (int)(tiles - rest); r.shares = (int)shares; r.ws = rest * shares * T::BM * T::BN * 4; }
+    return r;
+}
+LinPlan lin_plan(int64_t M, int64_t N, int64_t kbytes, bool wide) {
+    auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    const int64_t small = up(M, 128) * up(N, 128), big = up(M, 256) * up(N, 256);
+    if (M <= 64 || small < 64) return {ROWS, 0, 1, 0};
+    if (!wide && big >= 128) return rounds_of<Big>(BIG, up(M, 256), up(N, 256), kbytes, CUS);          // (widened fragments do not leave registers for the large tile)
+    return rounds_of<Small>(SMALL, up(M, 128), up(N, 128), kbytes, 2 * CUS);
+}
+
+template <class In, class Eo, class T> int launch_tiles(const LinArgs& p, const LinPlan& plan, float* ws, hipStream_t stream) {
+    const int tm = (p.M + T::BM - 1) / T::BM, tn = (p.N + T::BN - 1) / T::BN, rest = tm * tn - plan.whole;
+    const Rounds rd = {plan.whole, plan.shares, ws};
+    constexpr int LDS = 4 * T::SLOT;
+    if (plan.whole) {
+        if (LDS > 65536) SVD_ALLOW_LDS((linear_tile_kernel<In, Eo, T, false>), LDS);
+        hipLaunchKernelGGL((linear_tile_kernel<In, Eo, T, false>), dim3((unsigned)plan.whole), dim3(T::WAVES * 64), LDS, stream, p, tm, tn, rd);
+        SVD_CHECK_LAUNCH("linear_act");
+    }
+    if (rest) {
+        if (LDS > 65536) SVD_ALLOW_LDS((linear_tile_kernel<In, Eo, T, true>), LDS);
+        hipLaunchKernelGGL((linear_tile_kernel<In, Eo, T, true>), dim3((unsigned)(rest * plan.shares)), dim3(T::WAVES * 64), LDS, stream, p, tm, tn, rd);
+        SVD_CHECK_LAUNCH("linear_act");
+        hipLaunchKernelGGL((linear_join_kernel<Eo, T>), dim3((unsigned)(rest * T::TM)), dim3(T::WAVES * 64), 0, stream, p, tm, tn, rd);
+    }
+    SVD_CHECK_LAUNCH("linear_act");
+    return SVD_OK;
+}
+
+template <class In, class Eo> int launch(const LinArgs& p, void* ws, int64_t ws_bytes, hipStream_t stream) {
+    const LinPlan plan = lin_plan(p.M, p.N, p.kbytes, In::kWiden);
+    if (ws_bytes < plan.ws || (plan.ws && !ws) || ((uintptr_t)ws & 15)) return SVD_EINVAL;
     const uintptr_t pair = p.out_f32 ? (uintptr_t)p.Y & 7 : (uintptr_t)p.Y & 3, rpair = !p.R ? 0 : p.res_f32 ? (uintptr_t)p.R & 7 : (uintptr_t)p.R & 3;
     const bool aligned = !(((uintptr_t)p.X | (uintptr_t)p.W | p.ldx | p.ldw | p.kbytes) & 15) && !pair && !rpair && !((p.ldy | (p.R ? p.ldr : 0) | p.N) & 1) &&
                          p.ldx < (1 << 23) && p.ldw < (1 << 23);
-    if (p.M <= 64 || tiles(128, 128) < 64) {
+    if (plan.form == ROWS) {
         const int tm = p.M <= 32 ? 1 : 2;
         const int64_t tn = (p.N + 31) / 32, grid = (p.M + 32 * tm - 1) / (32 * tm) * tn;
         if (grid > 0x7fffffff) return SVD_EINVAL;
         if (tm == 1) hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 1>), dim3((unsigned)grid), dim3(512), 0, stream, p, (int)tn);
         else hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 2>), dim3((unsigned)grid), dim3(512), 0, stream, p, (int)tn);
     } else if (!aligned) {
-        const int64_t grid = tiles(128, 128);
+        const int64_t tn = (p.N + 127) / 128, grid = (int64_t)((p.M + 127) / 128) * tn;
         if (grid > 0x7fffffff) return SVD_EINVAL;
-        hipLaunchKernelGGL((linear_any_kernel<In, Eo>), dim3((unsigned)grid), dim3(256), 0, stream, p, (p.N + 127) / 128);
+        hipLaunchKernelGGL((linear_any_kernel<In, Eo>), dim3((unsigned)grid), dim3(256), 0, stream, p, (int)tn);
     } else {
-        bool big = false;
-        if constexpr (!In::kWiden) {          // (widened fragments do not leave registers for the large tile)
-            big = tiles(256, 256) >= 128;
-            if (big) {
-                if (tiles(256, 256) > 0x7fffffff) return SVD_EINVAL;
-                SVD_ALLOW_LDS((linear_tile_kernel<In, Eo, Big>), 4 * Big::SLOT);
-                hipLaunchKernelGGL((linear_tile_kernel<In, Eo, Big>), dim3((unsigned)tiles(256, 256)), dim3(512), 4 * Big::SLOT, stream, p, (p.M + 255) / 256, (p.N + 255) / 256);
-            }
-        }
-        if (!big) {
-            if (tiles(128, 128) > 0x7fffffff) return SVD_EINVAL;
-            hipLaunchKernelGGL((linear_tile_kernel<In, Eo, Small>), dim3((unsigned)tiles(128, 128)), dim3(256), 4 * Small::SLOT, stream, p, (p.M + 127) / 128, (p.N + 127) / 128);
-        }
+        if ((int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128) * 8 > 0x7fffffff) return SVD_EINVAL;
+        if constexpr (!In::kWiden)
+            if (plan.form == BIG) return launch_tiles<In, Eo, Big>(p, plan, (float*)ws, stream);
+        return launch_tiles<In, Eo, Small>(p, plan, (float*)ws, stream);
     }
     SVD_CHECK_LAUNCH("linear_act");
     return SVD_OK;
@@ -448,9 +538,15 @@ template <class In, class Eo> int launch(const LinArgs& p, hipStream_t stream) {
 
 }  // namespace
 
+extern "C" int64_t svd_linear_act_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t flags, int32_t in_dtype) {
+    if (M < 0 || M > 0x7fffff00 || N < 1 || N > 0x7fffff00 || K < 1 || K > 0x3fffff00) return SVD_EINVAL;
+    const bool f8 = in_dtype == SVD_DTYPE_F8;
+    return lin_plan(M, N, (int64_t)K * (f8 ? 1 : 2), f8 && (flags & SVD_LIN_OUT_F32)).ws;
+}
+
 extern "C" int svd_linear_act(const void* X, int64_t ldx, const void* W, int64_t ldw, const float* xscale, const float* wscale, const float* bias,
                               const void* R, int64_t ldr, void* Y, int64_t ldy, int64_t M, int32_t N, int32_t K, int32_t act, int32_t flags,
-                              int32_t in_dtype, int32_t dtype, svd_stream_t stream) {
+                              void* ws, int64_t ws_bytes, int32_t in_dtype, int32_t dtype, svd_stream_t stream) {
     const int es = in_dtype == SVD_DTYPE_F8 ? 1 : 2;
     if (!X || !W || !Y || M < 0 || M > 0x7fffff00 || N < 1 || N > 0x7fffff00 || K < 1 || K > 0x3fffff00 || ldx < K || ldw < K || ldy < N || (R && ldr < N)) return SVD_EINVAL;
     if (act < SVD_ACT_NONE || act > SVD_ACT_SILU || (flags & ~(SVD_LIN_RES_F32 | SVD_LIN_OUT_F32)) || (!R && (flags & SVD_LIN_RES_F32))) return SVD_EINVAL;
@@ -463,8 +559,8 @@ extern "C" int svd_linear_act(const void* X, int64_t ldx, const void* W, int64_t
     if (M == 0) return SVD_OK;
     const LinArgs p = {(const char*)X, ldx * es, (const char*)W, ldw * es, xscale, wscale, bias, R, ldr, Y, ldy, (int)M, N, K * es, act,
                        !!(flags & SVD_LIN_RES_F32), !!(flags & SVD_LIN_OUT_F32)};
-    if (in_dtype == SVD_DTYPE_F16) return launch<InF16, ElemF16>(p, (hipStream_t)stream);
-    if (in_dtype == SVD_DTYPE_BF16) return launch<InBF16, ElemBF16>(p, (hipStream_t)stream);
-    if (p.out_f32) return dtype == SVD_DTYPE_F16 ? launch<InF8Wide, ElemF16>(p, (hipStream_t)stream) : launch<InF8Wide, ElemBF16>(p, (hipStream_t)stream);
-    return dtype == SVD_DTYPE_F16 ? launch<InF8, ElemF16>(p, (hipStream_t)stream) : launch<InF8, ElemBF16>(p, (hipStream_t)stream);
+    if (in_dtype == SVD_DTYPE_F16) return launch<InF16, ElemF16>(p, ws, ws_bytes, (hipStream_t)stream);
+    if (in_dtype == SVD_DTYPE_BF16) return launch<InBF16, ElemBF16>(p, ws, ws_bytes, (hipStream_t)stream);
+    if (p.out_f32) return dtype == SVD_DTYPE_F16 ? launch<InF8Wide, ElemF16>(p, ws, ws_bytes, (hipStream_t)stream) : launch<InF8Wide, ElemBF16>(p, ws, ws_bytes, (hipStream_t)stream);
+    return dtype == SVD_DTYPE_F16 ? launch<InF8, ElemF16>(p, ws, ws_bytes, (hipStream_t)stream) : launch<InF8, ElemBF16>(p, ws, ws_bytes, (hipStream_t)stream);
 }

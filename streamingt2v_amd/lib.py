@@ -42,7 +42,7 @@ SYMBOLS = [
     "svd_attn_cross_d64", "svd_adaptive_avgpool_tokens", "svd_i2v_image_temporal_encoder", "svd_ddim_cfg_step", "svd_frames_to_uint8", "svd_gelu_rows",
     "svd_ff_geglu_fused", "svd_ff_fused_pack_bytes", "svd_rowgemm320", "svd_rowgemm320_pack_bytes", "svd_rowproj320", "svd_rowproj320_pack_bytes",
     "svd_prelu_rows", "svd_dwconv3x3_gelu", "svd_window_attn_7x7", "svd_warp_bilinear", "svd_resize_bilinear_f32", "svd_vfi_merge", "svd_vfi_tta_average",
-    "svd_rmsnorm", "svd_linear_act", "svd_attn_diff", "svd_attn_diff_ws_bytes",
+    "svd_rmsnorm", "svd_linear_act", "svd_linear_act_ws_bytes", "svd_attn_diff", "svd_attn_diff_ws_bytes",
 ]
 
 A_PLAIN, A_CONV3X3, A_TEMPORAL3 = 0, 1, 2
@@ -157,13 +157,15 @@ def _load():
     lib.svd_vfi_merge.argtypes = [vp, vp, vp, i64, vp, i64, vp, vp, i64, vp]
     lib.svd_vfi_tta_average.argtypes = [vp, vp, vp, i32, i32, vp]
     lib.svd_rmsnorm.argtypes = [vp, i64, vp, i64, vp, f32, vp, i64, vp, vp, i64, i64, i32, i32, i32, vp]
-    lib.svd_linear_act.argtypes = [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, i64, i64, i32, i32, i32, i32, i32, i32, vp]
+    lib.svd_linear_act_ws_bytes.restype = C.c_int64
+    lib.svd_linear_act_ws_bytes.argtypes = [i64, i32, i32, i32, i32]
+    lib.svd_linear_act.argtypes = [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, i64, i64, i32, i32, i32, i32, vp, i64, i32, i32, vp]
     lib.svd_attn_diff_ws_bytes.restype = C.c_int64
     lib.svd_attn_diff_ws_bytes.argtypes = [i32] * 5
     lib.svd_attn_diff.argtypes = [vp, i64, i64, i64] * 4 + [vp, f32, vp, f32, vp, vp, i32, i32, i32, i32, i32, i32, vp, i64, i32, vp]
     for s in SYMBOLS:
         fn = getattr(lib, s)
-        if s not in ("svd_last_error", "svd_groupnorm_partial_elems", "svd_ff_fused_pack_bytes", "svd_rowgemm320_pack_bytes", "svd_rowproj320_pack_bytes", "svd_attn_diff_ws_bytes"):
+        if s not in ("svd_last_error", "svd_groupnorm_partial_elems", "svd_ff_fused_pack_bytes", "svd_rowgemm320_pack_bytes", "svd_rowproj320_pack_bytes", "svd_attn_diff_ws_bytes", "svd_linear_act_ws_bytes"):
             fn.restype = C.c_int
     if lib.svd_abi_version() != ABI_VERSION:
         raise ImportError(f"libsvdhip.so ABI {lib.svd_abi_version()} != binding ABI {ABI_VERSION}; rebuild")

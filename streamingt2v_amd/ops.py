@@ -1025,9 +1025,12 @@ def linear_act(x, w, *, bias=None, act=None, residual=None, x_scale=None, w_scal
     if worklog is not None:
         _wl("linear_act", 2.0 * M * N * K, float(M + N) * K * x.element_size() + float(M) * N * (y.element_size() + (residual.element_size() if residual is not None else 0)))
     if M:
+        it = _l.DTYPE_F8 if f8 else _DT[e]
+        need = _lib.svd_linear_act_ws_bytes(M, N, K, flags, it) if M > 64 else 0
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None          # from the allocator, per call: its stream and its graph's pool own it
         check(_lib.svd_linear_act(x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), x_scale.data_ptr() if x_scale is not None else None,
                                   w_scale.data_ptr() if w_scale is not None else None, bias.data_ptr() if bias is not None else None, r_ptr, ldr, y.data_ptr(),
-                                  _ld(y), M, N, K, _l.ACT[act], flags, _l.DTYPE_F8 if f8 else _DT[e], _DT[e], torch.cuda.current_stream().cuda_stream), "svd_linear_act")
+                                  _ld(y), M, N, K, _l.ACT[act], flags, ws.data_ptr() if need else None, need, it, _DT[e], torch.cuda.current_stream().cuda_stream), "svd_linear_act")
     return y
 
 

@@ -32,8 +32,8 @@ def test_rmsnorm_no_rows(lib):
     assert norm(lib, rows=0) == OK
 
 
-def linear(lib, X=A, ldx=64, W=A, ldw=64, xs=None, ws=None, bias=None, R=None, ldr=0, Y=A, ldy=32, M=4, N=32, K=64, act=0, flags=0, it=F16, dt=F16):
-    return lib.svd_linear_act(X, ldx, W, ldw, xs, ws, bias, R, ldr, Y, ldy, M, N, K, act, flags, it, dt, None)
+def linear(lib, X=A, ldx=64, W=A, ldw=64, xs=None, ws=None, bias=None, R=None, ldr=0, Y=A, ldy=32, M=4, N=32, K=64, act=0, flags=0, scratch=None, sb=0, it=F16, dt=F16):
+    return lib.svd_linear_act(X, ldx, W, ldw, xs, ws, bias, R, ldr, Y, ldy, M, N, K, act, flags, scratch, sb, it, dt, None)
 
 
 @pytest.mark.parametrize("bad", [
@@ -42,6 +42,17 @@ def linear(lib, X=A, ldx=64, W=A, ldw=64, xs=None, ws=None, bias=None, R=None, l
     dict(W=A + 1), dict(Y=A + 1), dict(Y=A + 2, flags=2), dict(R=A + 2, ldr=32, flags=1)], ids=str)
 def test_linear_refuses(lib, bad):
     assert linear(lib, **bad) == EINVAL
+
+
+def test_linear_scratch_size(lib):
+    f = lib.svd_linear_act_ws_bytes
+    assert f(-1, 1, 1, 0, F16) == EINVAL and f(1, 0, 1, 0, F16) == EINVAL and f(1, 1, 0, 0, F16) == EINVAL
+    assert f(0, 64, 64, 0, F16) == 0 and f(1, 5120, 1280, 0, F8) == 0 and f(64, 64, 64, 0, F16) == 0
+    for m, n, k, it, fl in [(28800, 1280, 5120, BF16, 0), (2304, 1280, 5120, F8, 0), (2304, 1280, 5120, F8, 2), (1100, 1040, 4096, F16, 0)]:
+        need = f(m, n, k, fl, it)
+        assert 0 < need <= 1 << 29 and need % 16 == 0
+        big = dict(M=m, N=n, K=k, ldx=k, ldw=k, ldy=n, it=it, flags=fl, dt=BF16 if it != F16 else F16)
+        assert linear(lib, **big) == EINVAL and linear(lib, scratch=A, sb=need - 1, **big) == EINVAL and linear(lib, scratch=A + 8, sb=need, **big) == EINVAL
 
 
 def test_linear_no_rows(lib):

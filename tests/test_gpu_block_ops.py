@@ -227,7 +227,8 @@ def test_linear_activations_reach_far_values(ops, act, t):
 
 
 @pytest.mark.parametrize("t", [F16, BF16, F8], ids=str)
-@pytest.mark.parametrize("m,n,k", [(3, 272, 208), (70, 272, 208), (300, 272, 208), (1100, 1040, 208), (1100, 1041, 209), (1100, 1040, 80), (4100, 2064, 208), (4100, 2064, 64), (4096, 2048, 320)])
+@pytest.mark.parametrize("m,n,k", [(3, 272, 208), (70, 272, 208), (300, 272, 208), (1100, 1040, 208), (1100, 1041, 209), (1100, 1040, 80), (4100, 2064, 208), (4100, 2064, 64), (4096, 2048, 320), (1100, 1040, 2064),
+                                   (8448, 2176, 1120)])
 def test_linear_picks_rows_and_columns(ops, t, m, n, k):
     """One-hot rows select columns of W: any swapped lane, row or K chunk shows as another number, exactly.  Few rows, 128- and 256-row tiles, unaligned rows, one to
     many K steps with and without a rest."""
