@@ -164,13 +164,14 @@ template <class In, class Eo> __global__ __launch_bounds__(256) void linear_any_
 }
 
 // ---- large products: BM x BN outputs per workgroup of WM x WN waves, each TM x TN tiles of 32 x 32; rows 16-byte aligned ----
-// K goes in steps of 64 bytes through a ring of four LDS slots (rows of 64 bytes, 16-byte chunks swizzled by (row >> 2) & 3: 16 lanes that read one chunk of 16
-// rows touch all 64 banks once), filled by LDS-DMA three steps ahead.  A step multiplies fragments that the step before has read and reads the next step's between its
-// matrix instructions; the one barrier per step only says that a slot may be filled again.
+// K goes in steps of 128 bytes (whole cache lines: with 64 the L2 has twice the requests to serve) through two LDS slots, rows of 128 bytes with 16-byte chunks
+// swizzled by (row >> 1) & 7: 16 lanes that read one chunk of 16 rows touch all 64 banks once.  A half step of 64 bytes multiplies fragments that the half before has read
+// and reads the next half's between its matrix instructions.  So a slot is free when the first half of its step is done, and is filled then, by LDS-DMA, for the
+// step after the next: two halves of a step (2000 cycles of matrix work) ahead of its use, one barrier a step.
 // W's rows lie in LDS as even, then odd columns of each 64: a lane's two tiles of such a block are two adjacent columns, so results leave (and residuals come) as
 // pairs, 32 lanes a contiguous 128 (fp32: 256) bytes of a row.
 template <int WM_, int WN_, int TM_, int TN_> struct Tile {
-    static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, WAVES = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32, SLOT = (BM + BN) * 64, REQ = (BM + BN) / 16 / WAVES;
+    static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, WAVES = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32, SLOT = (BM + BN) * 128, REQ = (BM + BN) / 8 / WAVES;
 };
 __device__ const uint4 g_zeros = {0, 0, 0, 0};
 
@@ -266,7 +267,7 @@ template <class In, class Eo, class T, bool SHARE> __global__ __launch_bounds__(
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const uint32_t lds = lds_addr_of(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l31 = lane & 31, hi = lane >> 5;
-    int m0, n0, k_from = 0, steps = (p.kbytes + 63) >> 6;          // steps of 64 bytes of K
+    int m0, n0, k_from = 0, steps = (p.kbytes + 127) >> 7;          // steps of 128 bytes of K
     {
         int w;
         if constexpr (!SHARE) {          // consecutive workgroups go round the 8 XCDs: each gets a contiguous piece of the list
@@ -282,29 +283,28 @@ template <class In, class Eo, class T, bool SHARE> __global__ __launch_bounds__(
         m0 *= T::BM; n0 *= T::BN;
     }
     const int wm = (wave / T::WN) * TM * 32, wn = (wave % T::WN) * TN * 32;
-    // requests: 16 rows of 64 bytes each; a wave's are all of X or all of W
-    constexpr int X_REQ = T::BM / 16;
-    const bool is_x = wave * T::REQ < X_REQ;
-    const char* src = (is_x ? p.X + (int64_t)m0 * p.ldx : p.W + (int64_t)n0 * p.ldw) + (int64_t)k_from * 64;
-    const int kbytes = p.kbytes - k_from * 64;
-    const int chunk = (lane & 3) ^ ((lane >> 4) & 3);
+    // requests: 8 rows of 128 bytes each; a wave's are all of X or all of W
+    const bool is_x = wave * T::REQ < T::BM / 8;
+    const char* src = (is_x ? p.X + (int64_t)m0 * p.ldx : p.W + (int64_t)n0 * p.ldw) + (int64_t)k_from * 128;
+    const int kbytes = p.kbytes - k_from * 128;
+    const int chunk = (lane & 7) ^ (lane >> 4);          // of the even requests; the odd ones' differs in bit 2
     uint32_t off[T::REQ];
 #pragma unroll
     for (int u = 0; u < T::REQ; ++u) {
-        const int r = (wave * T::REQ + u) * 16 + (lane >> 2) - (is_x ? 0 : T::BM);
+        const int r = (wave * T::REQ + u) * 8 + (lane >> 3) - (is_x ? 0 : T::BM);
         const int n = (r & ~63) | ((r & 31) << 1) | ((r >> 5) & 1);
         const int row = is_x ? min(r, p.M - 1 - m0) : min(n, p.N - 1 - n0);          // rows behind the last repeat it; their results are not stored
-        off[u] = (uint32_t)row * (uint32_t)(is_x ? p.ldx : p.ldw) + chunk * 16;
+        off[u] = (uint32_t)row * (uint32_t)(is_x ? p.ldx : p.ldw) + (chunk ^ (u & 1) << 2) * 16;
     }
     auto request = [&](int j) {
-        const uint32_t dst = lds + (j & 3) * T::SLOT + wave * T::REQ * 1024;
-        if (__builtin_expect(j * 64 + 64 <= kbytes, 1)) {
+        const uint32_t dst = lds + (j & 1) * T::SLOT + wave * T::REQ * 1024;
+        if (__builtin_expect(j * 128 + 128 <= kbytes, 1)) {
 #pragma unroll
-            for (int u = 0; u < T::REQ; ++u) glds16_saddr(off[u], src + j * 64, __builtin_amdgcn_readfirstlane(dst + u * 1024));
+            for (int u = 0; u < T::REQ; ++u) glds16_saddr(off[u], src + (int64_t)j * 128, __builtin_amdgcn_readfirstlane(dst + u * 1024));
         } else {          // the last step's chunks behind K are zeros
 #pragma unroll
             for (int u = 0; u < T::REQ; ++u)
-                glds16_asm(j * 64 + chunk * 16 < kbytes ? src + j * 64 + off[u] : (const char*)&g_zeros, __builtin_amdgcn_readfirstlane(dst + u * 1024));
+                glds16_asm(j * 128 + (chunk ^ (u & 1) << 2) * 16 < kbytes ? src + (int64_t)j * 128 + off[u] : (const char*)&g_zeros, __builtin_amdgcn_readfirstlane(dst + u * 1024));
         }
     };
     f32x16_t acc[TM * TN];
@@ -313,29 +313,27 @@ template <class In, class Eo, class T, bool SHARE> __global__ __launch_bounds__(
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
     uint4 f[2][NF][2];
-    const uint32_t la = l31 * 64 + (((2 * hi) ^ ((l31 >> 2) & 3)) << 4);
-    auto read = [&](int j, int set, int e) {          // fragment e: X tiles 0 .. TM - 1, then W tiles
-        const uint32_t at = lds + (j & 3) * T::SLOT + (e < TM ? (wm + 32 * e) * 64 : (T::BM + wn + 32 * (e - TM)) * 64) + la;
+    const uint32_t la = l31 * 128 + (((2 * hi) ^ ((l31 >> 1) & 7)) << 4);
+    auto read = [&](int j, int half, int e) {          // fragment e of half a step: X tiles 0 .. TM - 1, then W tiles
+        const uint32_t at = (lds + (j & 1) * T::SLOT + (e < TM ? (wm + 32 * e) * 128 : (T::BM + wn + 32 * (e - TM)) * 128) + la) ^ (half * 64);
         typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-        f[set][e][0] = __builtin_bit_cast(uint4, *(const __attribute__((address_space(3))) u32x4_t*)at);
-        f[set][e][1] = __builtin_bit_cast(uint4, *(const __attribute__((address_space(3))) u32x4_t*)(at ^ 16));
+        f[half][e][0] = __builtin_bit_cast(uint4, *(const __attribute__((address_space(3))) u32x4_t*)at);
+        f[half][e][1] = __builtin_bit_cast(uint4, *(const __attribute__((address_space(3))) u32x4_t*)(at ^ 16));
     };
     // the order in which a step's fragments are read for the next: first those that its first products take
     auto nth = [](int e) { return e == 0 ? 0 : e <= TN ? TM + e - 1 : e - TN; };
     if (steps > 0) request(0);
     if (steps > 1) request(1);
-    if (steps > 2) request(2);
     svd_wait_dma();
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < NF; ++e) read(0, 0, e);
-    auto step = [&]<int SET>(int j) {
-        if (__builtin_expect(j + 2 < steps, 1)) {          // all but the last request: step j + 1 is there
-            if constexpr (T::REQ == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-            else svd_wait_dma();
-        } else svd_wait_dma();
-        __syncthreads();
-        if (j + 3 < steps) request(j + 3);          // into the slot whose fragments were read in step j - 2
+    auto half_step = [&]<int SET>(int j) {
+        if constexpr (SET == 1) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");          // step j + 1 is there; this wave's reads of step j are done
+            __syncthreads();
+            if (j + 2 < steps) request(j + 2);
+        }
         constexpr int PASSES = In::kWiden ? 4 : In::kBytes == 1 ? 1 : 2;          // matrix instructions per tile and step
         int e = 0;
 #pragma unroll
@@ -344,7 +342,7 @@ template <class In, class Eo, class T, bool SHARE> __global__ __launch_bounds__(
             for (int i = 0; i < TM; ++i)
 #pragma unroll
                 for (int n = 0; n < TN; ++n) {
-                    if (e < NF) read(j + 1, SET ^ 1, nth(e));
+                    if (e < NF) read(j + SET, SET ^ 1, nth(e));
                     ++e;
                     const uint4 *a = f[SET][i], *b = f[SET][TM + n];
                     f32x16_t& c = acc[i * TN + n];
@@ -363,9 +361,10 @@ template <class In, class Eo, class T, bool SHARE> __global__ __launch_bounds__(
                     __builtin_amdgcn_sched_barrier(0);
                 }
     };
-    for (int j = 0; j < steps; j += 2) {
-        step.template operator()<0>(j);
-        if (j + 1 < steps) step.template operator()<1>(j + 1);
+#pragma unroll 1
+    for (int j = 0; j < steps; ++j) {
+        half_step.template operator()<0>(j);
+        half_step.template operator()<1>(j);
     }
 
     if constexpr (SHARE) {          // the sums, as they lie
@@ -475,10 +474,10 @@ constexpr int CUS = 256;
 enum { ROWS, BIG, SMALL };
 struct LinPlan { int form, whole, shares; int64_t ws; };
 template <class T> LinPlan rounds_of(int form, int64_t tm, int64_t tn, int64_t kbytes, int slots) {
-    const int64_t tiles = tm * tn, rest = tiles % slots, steps = (kbytes + 63) / 64;
+    const int64_t tiles = tm * tn, rest = tiles % slots, steps = (kbytes + 127) / 128;
     LinPlan r = {form, (int)tiles, 1, 0};
     int64_t shares = rest ? slots / rest : 1;
-    if (shares > steps / 8) shares = steps / 8;          // a share of at least 8 steps
+    if (shares > steps / 4) shares = steps / 4;          // a share of at least 4 steps
     if (shares > 8) shares = 8;
     if (shares > 1) { r.whole = (int)(tiles - rest); r.shares = (int)shares; r.ws = rest * shares * T::BM * T::BN * 4; }
     return r;
@@ -494,7 +493,7 @@ LinPlan lin_plan(int64_t M, int64_t N, int64_t kbytes, bool wide) {
 template <class In, class Eo, class T> int launch_tiles(const LinArgs& p, const LinPlan& plan, float* ws, hipStream_t stream) {
     const int tm = (p.M + T::BM - 1) / T::BM, tn = (p.N + T::BN - 1) / T::BN, rest = tm * tn - plan.whole;
     const Rounds rd = {plan.whole, plan.shares, ws};
-    constexpr int LDS = 4 * T::SLOT;
+    constexpr int LDS = 2 * T::SLOT;
     if (plan.whole) {
         if (LDS > 65536) SVD_ALLOW_LDS((linear_tile_kernel<In, Eo, T, false>), LDS);
         hipLaunchKernelGGL((linear_tile_kernel<In, Eo, T, false>), dim3((unsigned)plan.whole), dim3(T::WAVES * 64), LDS, stream, p, tm, tn, rd);
