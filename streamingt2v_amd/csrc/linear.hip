@@ -214,39 +214,43 @@ template <class Eo, int TM, int TN> __device__ __forceinline__ void finish_tiles
     else if (p.act == SVD_ACT_GELU) act_all<SVD_ACT_GELU>(acc);
     else if (p.act == SVD_ACT_GELU_TANH) act_all<SVD_ACT_GELU_TANH>(acc);
     else if (p.act == SVD_ACT_SILU) act_all<SVD_ACT_SILU>(acc);
+    // Addresses: the row is the wave's (scalars), a lane adds its column pair and, in the upper half, four rows, in 32 bits.
+    const int ey = p.out_f32 ? 4 : 2, er = p.res_f32 ? 4 : 2;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int b = 0; b < TN / 2; ++b) {
-            const int n = n0 + 64 * b + 2 * l31, mb = m0 + 32 * i + 4 * hi;
+            const int n = n0 + 64 * b + 2 * l31, mb = m0 + 32 * i;
             f32x16_t &v0 = acc[i * TN + 2 * b], &v1 = acc[i * TN + 2 * b + 1];
             if (n >= p.N) continue;
             if (p.R) {
+                const char* base = (const char*)p.R + ((int64_t)mb * p.ldr + n0 + 64 * b) * er;
+                const uint32_t lane_off = (4 * hi * (uint32_t)p.ldr + 2 * l31) * er;
 #pragma unroll
                 for (int half = 0; half < 16; half += 8) {          // eight rows' residuals in flight
                     float2 res[16];
 #pragma unroll
                     for (int r = half; r < half + 8; ++r) {
-                        const int64_t at = (int64_t)min(mb + 8 * (r >> 2) + (r & 3), p.M - 1) * p.ldr + n;
-                        if (p.res_f32) res[r] = *(const float2*)((const float*)p.R + at);
-                        else { const uint32_t w = *(const uint32_t*)((const uint16_t*)p.R + at); res[r] = make_float2(Eo::lo(w), Eo::hi(w)); }
+                        const int row = 8 * (r >> 2) + (r & 3);
+                        const char* at = whole ? base + (int64_t)row * p.ldr * er + lane_off
+                                               : (const char*)p.R + ((int64_t)min(mb + row + 4 * hi, p.M - 1) * p.ldr + n) * er;
+                        if (p.res_f32) res[r] = *(const float2*)at;
+                        else { const uint32_t w = *(const uint32_t*)at; res[r] = make_float2(Eo::lo(w), Eo::hi(w)); }
                     }
 #pragma unroll
                     for (int r = half; r < half + 8; ++r) { v0[r] += res[r].x; v1[r] += res[r].y; }
                 }
             }
-            auto store = [&](int r) {
-                const int64_t at = (int64_t)(mb + 8 * (r >> 2) + (r & 3)) * p.ldy + n;
-                if (p.out_f32) *(float2*)((float*)p.Y + at) = make_float2(v0[r], v1[r]);
-                else *(uint32_t*)((uint16_t*)p.Y + at) = Eo::pack(v0[r], v1[r]);
-            };
-            if (whole) {
+            char* base = (char*)p.Y + ((int64_t)mb * p.ldy + n0 + 64 * b) * ey;
+            const uint32_t lane_off = (4 * hi * (uint32_t)p.ldy + 2 * l31) * ey;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) store(r);
-            } else {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (mb + 8 * (r >> 2) + (r & 3) < p.M) store(r);
+            for (int r = 0; r < 16; ++r) {
+                const int row = 8 * (r >> 2) + (r & 3);
+                char* at = base + (int64_t)row * p.ldy * ey + lane_off;
+                if (whole || mb + row + 4 * hi < p.M) {
+                    if (p.out_f32) *(float2*)at = make_float2(v0[r], v1[r]);
+                    else *(uint32_t*)at = Eo::pack(v0[r], v1[r]);
+                }
             }
         }
 }
@@ -385,7 +389,7 @@ template <class In, class Eo, class T, bool SHARE> __global__ __launch_bounds__(
 // One workgroup per split tile and band of 32 rows of its waves: the shares' sums in their order, then the epilogue.
 template <class Eo, class T> __global__ __launch_bounds__(T::WAVES * 64) void linear_join_kernel(LinArgs p, int tiles_m, int tiles_n, Rounds rd) {
     __shared__ float s_xs[T::WAVES][32];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, t = blockIdx.x / T::TM, i = blockIdx.x % T::TM;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), t = blockIdx.x / T::TM, i = blockIdx.x % T::TM;
     int m0, n0;
     tile_place(rd.whole + t, tiles_m, tiles_n, m0, n0);
     m0 = m0 * T::BM + (wave / T::WN) * T::TM * 32 + 32 * i;
@@ -514,7 +518,7 @@ template <class In, class Eo> int launch(const LinArgs& p, void* ws, int64_t ws_
     if (ws_bytes < plan.ws || (plan.ws && !ws) || ((uintptr_t)ws & 15)) return SVD_EINVAL;
     const uintptr_t pair = p.out_f32 ? (uintptr_t)p.Y & 7 : (uintptr_t)p.Y & 3, rpair = !p.R ? 0 : p.res_f32 ? (uintptr_t)p.R & 7 : (uintptr_t)p.R & 3;
     const bool aligned = !(((uintptr_t)p.X | (uintptr_t)p.W | p.ldx | p.ldw | p.kbytes) & 15) && !pair && !rpair && !((p.ldy | (p.R ? p.ldr : 0) | p.N) & 1) &&
-                         p.ldx < (1 << 23) && p.ldw < (1 << 23);
+                         p.ldx < (1 << 23) && p.ldw < (1 << 23) && p.ldy < (1 << 26) && p.ldr < (1 << 26);          // tiles are addressed with 32-bit offsets
     if (plan.form == ROWS) {
         const int tm = p.M <= 32 ? 1 : 2;
         const int64_t tn = (p.N + 31) / 32, grid = (p.M + 32 * tm - 1) / (32 * tm) * tn;
