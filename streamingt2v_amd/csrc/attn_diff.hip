@@ -459,21 +459,49 @@ template <class E> __global__ __launch_bounds__(64, 2) void attn_diff_wave_kerne
     if (w.hi == 0) *(float4*)(part + 256) = make_float4(w.m[0], w.l[0], w.m[1], w.l[1]);
 }
 
-// One wave per row: lane = two channels.  The shares join in their order, so the result does not depend on which finished first.
-template <class E> __global__ __launch_bounds__(64) void attn_diff_join_kernel(DiffArgs p, int shares, const float* ws) {
-    const int lane = threadIdx.x, rows = p.n_q * p.group, row = blockIdx.x % rows, bh = blockIdx.x / rows, h = bh % p.kv_heads, b = bh / p.kv_heads;
+// One workgroup per row: lane = two channels, the four waves take the shares in turn, four requested at once, and meet in LDS.  The order of the sums is fixed, so the result
+// does not depend on which share finished first.  (One wave and one share at a time: 11.6 us for 128 rows of 32 shares, 7.8 for 8 of 17.)
+template <class E> __global__ __launch_bounds__(256) void attn_diff_join_kernel(DiffArgs p, int shares, const float* ws) {
+    __shared__ float s_m[4][2], s_l[4][2], s_o[4][4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int rows = p.n_q * p.group, row = blockIdx.x % rows, bh = blockIdx.x / rows, h = bh % p.kv_heads, b = bh / p.kv_heads;
     const float* part = ws + (int64_t)blockIdx.x * shares * PART;
-    float m[2] = {M_NONE, M_NONE};
-    for (int s = lane; s < shares; s += 64) { m[0] = fmaxf(m[0], part[s * PART + 256]); m[1] = fmaxf(m[1], part[s * PART + 258]); }
-    m[0] = wave_max(m[0]); m[1] = wave_max(m[1]);
-    float l[2] = {0.f, 0.f}, o[2][2] = {};
-    for (int s = 0; s < shares; ++s) {
-        const float4 ml = *(const float4*)(part + s * PART + 256);
-        const float a0 = __builtin_amdgcn_exp2f(ml.x - m[0]), a1 = __builtin_amdgcn_exp2f(ml.z - m[1]);
-        l[0] = fmaf(ml.y, a0, l[0]); l[1] = fmaf(ml.w, a1, l[1]);
-        const float2 x = *(const float2*)(part + s * PART + 2 * lane), y = *(const float2*)(part + s * PART + 128 + 2 * lane);
-        o[0][0] = fmaf(x.x, a0, o[0][0]); o[0][1] = fmaf(x.y, a0, o[0][1]);
-        o[1][0] = fmaf(y.x, a1, o[1][0]); o[1][1] = fmaf(y.y, a1, o[1][1]);
+    float m[2] = {M_NONE, M_NONE}, l[2] = {0.f, 0.f}, o[2][2] = {};
+    for (int s0 = wave; s0 < shares; s0 += 16) {
+        float4 ml[4];
+        float2 x[4], y[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float* at = part + (int64_t)min(s0 + 4 * u, shares - 1) * PART;
+            ml[u] = *(const float4*)(at + 256);
+            x[u] = *(const float2*)(at + 2 * lane);
+            y[u] = *(const float2*)(at + 128 + 2 * lane);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (s0 + 4 * u >= shares) break;
+            const float m0 = fmaxf(m[0], ml[u].x), m1 = fmaxf(m[1], ml[u].z);
+            const float a0 = __builtin_amdgcn_exp2f(m[0] - m0), a1 = __builtin_amdgcn_exp2f(m[1] - m1), b0 = __builtin_amdgcn_exp2f(ml[u].x - m0), b1 = __builtin_amdgcn_exp2f(ml[u].z - m1);
+            m[0] = m0; m[1] = m1;
+            l[0] = fmaf(l[0], a0, ml[u].y * b0); l[1] = fmaf(l[1], a1, ml[u].w * b1);
+            o[0][0] = fmaf(o[0][0], a0, x[u].x * b0); o[0][1] = fmaf(o[0][1], a0, x[u].y * b0);
+            o[1][0] = fmaf(o[1][0], a1, y[u].x * b1); o[1][1] = fmaf(o[1][1], a1, y[u].y * b1);
+        }
+    }
+    if (lane == 0) { s_m[wave][0] = m[0]; s_m[wave][1] = m[1]; s_l[wave][0] = l[0]; s_l[wave][1] = l[1]; }
+    s_o[wave][0][lane] = o[0][0]; s_o[wave][1][lane] = o[0][1]; s_o[wave][2][lane] = o[1][0]; s_o[wave][3][lane] = o[1][1];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        m[i] = fmaxf(fmaxf(s_m[0][i], s_m[1][i]), fmaxf(s_m[2][i], s_m[3][i]));
+        l[i] = o[i][0] = o[i][1] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float a = __builtin_amdgcn_exp2f(s_m[w][i] - m[i]);
+            l[i] = fmaf(s_l[w][i], a, l[i]);
+            o[i][0] = fmaf(s_o[w][2 * i][lane], a, o[i][0]); o[i][1] = fmaf(s_o[w][2 * i + 1][lane], a, o[i][1]);
+        }
     }
     const float lam = diff_lambda(p.lam, p.lambda_init, lane);
     const float w0 = l[0] == 0.f ? 0.f : 1.f / l[0], w1 = l[1] == 0.f ? 0.f : lam / l[1];
@@ -539,7 +567,7 @@ extern "C" int svd_attn_diff(const svd_bf16* Q, int64_t q_sb, int64_t q_st, int6
         SVD_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((attn_diff_wave_kernel<E>), dim3((unsigned)grid), dim3(64), LDS, (hipStream_t)stream, p, plan.row_blocks, plan.shares, (float*)ws));
         SVD_CHECK_LAUNCH("attn_diff");
         if (plan.shares > 1)
-            SVD_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((attn_diff_join_kernel<E>), dim3((unsigned)(batch * heads * n_q)), dim3(64), 0, (hipStream_t)stream, p, plan.shares, (const float*)ws));
+            SVD_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((attn_diff_join_kernel<E>), dim3((unsigned)((int64_t)batch * heads * n_q)), dim3(256), 0, (hipStream_t)stream, p, plan.shares, (const float*)ws));
     }
     SVD_CHECK_LAUNCH("attn_diff");
     return SVD_OK;

@@ -939,8 +939,15 @@ def _ld(t):
 
 def _on(x, *others):
     """Every tensor on x's GPU."""
-    assert x.is_cuda and all(t is None or t.device == x.device for t in others), "all tensors must be on one GPU"
-    return x.device
+    dev = x.device
+    assert x.is_cuda, "there is no form for host tensors"
+    for t in others:
+        assert t is None or t.device == dev, "all tensors must be on one GPU"
+    return dev
+
+
+# handle of the device's current stream (the stream object that torch.cuda.current_stream builds costs 2.6 us, a fifth of a one-token call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _vec(t, n):
@@ -965,23 +972,23 @@ def rmsnorm(x, gamma=None, *, eps=1e-6, residual=None, f8=False, out=None, out_s
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return rmsnorm(x, gamma, eps=eps, residual=residual, f8=f8, out=out, out_sum=out_sum)
-    y = out if out is not None else torch.empty((rows, Cc), dtype=F8 if f8 else e, device=dev)
+    y = out if out is not None else x.new_empty((rows, Cc), dtype=F8 if f8 else e)
     flags, scale, s, r_ptr, ldr, s_ptr, lds = 0, None, None, None, 0, None, 0
     if x.dtype == torch.float32:
         flags |= _l.RMS_X_F32
     if residual is not None:
-        s = out_sum if out_sum is not None else torch.empty((rows, Cc), dtype=residual.dtype, device=dev)
+        s = out_sum if out_sum is not None else x.new_empty((rows, Cc), dtype=residual.dtype)
         r_ptr, ldr, s_ptr, lds = residual.data_ptr(), _ld(residual), s.data_ptr(), _ld(s)
         if residual.dtype == torch.float32:
             flags |= _l.RMS_R_F32
     if f8:
         flags |= _l.RMS_OUT_F8
-        scale = torch.empty(rows, dtype=torch.float32, device=dev)
+        scale = x.new_empty(rows, dtype=torch.float32)
     if worklog is not None:
         _wl("rmsnorm", 6.0 * rows * Cc, float(rows) * Cc * (x.element_size() + y.element_size() + (2 * s.element_size() if s is not None else 0)))
     if rows:
         check(_lib.svd_rmsnorm(x.data_ptr(), _ld(x), r_ptr, ldr, gamma.data_ptr() if gamma is not None else None, eps, y.data_ptr(), _ld(y),
-                               scale.data_ptr() if f8 else None, s_ptr, lds, rows, Cc, flags, _DT[e], torch.cuda.current_stream().cuda_stream), "svd_rmsnorm")
+                               scale.data_ptr() if f8 else None, s_ptr, lds, rows, Cc, flags, _DT[e], _raw_stream(dev.index)), "svd_rmsnorm")
     if f8:
         return (y, scale) if s is None else (y, scale, s)
     return y if s is None else (y, s)
@@ -1015,7 +1022,7 @@ def linear_act(x, w, *, bias=None, act=None, residual=None, x_scale=None, w_scal
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return linear_act(x, w, bias=bias, act=act, residual=residual, x_scale=x_scale, w_scale=w_scale, out_dtype=out_dtype, out=out)
-    y = out if out is not None else torch.empty((M, N), dtype=out_dtype, device=dev)
+    y = out if out is not None else x.new_empty((M, N), dtype=out_dtype)
     flags = _l.LIN_OUT_F32 if out_dtype == torch.float32 else 0
     r_ptr, ldr = None, 0
     if residual is not None:
@@ -1030,14 +1037,17 @@ def linear_act(x, w, *, bias=None, act=None, residual=None, x_scale=None, w_scal
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None          # from the allocator, per call: its stream and its graph's pool own it
         check(_lib.svd_linear_act(x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), x_scale.data_ptr() if x_scale is not None else None,
                                   w_scale.data_ptr() if w_scale is not None else None, bias.data_ptr() if bias is not None else None, r_ptr, ldr, y.data_ptr(),
-                                  _ld(y), M, N, K, _l.ACT[act], flags, ws.data_ptr() if need else None, need, it, _DT[e], torch.cuda.current_stream().cuda_stream), "svd_linear_act")
+                                  _ld(y), M, N, K, _l.ACT[act], flags, ws.data_ptr() if need else None, need, it, _DT[e], _raw_stream(dev.index)), "svd_linear_act")
     return y
 
 
 def _strides4(t):
-    """(sequence, token, head) strides of [batch, n, heads, 128]; a dimension of one has none."""
-    assert t.stride(3) == 1, "a head's 128 channels must be contiguous"
-    return [st if n > 1 else 0 for n, st in zip(t.shape[:3], t.stride()[:3])]
+    """(sequence, token, head) strides of [batch, n, heads, 128]; a dimension of one has none that counts."""
+    b, n, h, c = t.stride()
+    assert c == 1, "a head's 128 channels must be contiguous"
+    if (b | n | h) & 7 or n > 1 << 25:
+        b, n, h = (st if size > 1 else 0 for size, st in zip(t.shape, (b, n, h)))
+    return b, n, h
 
 
 def attn_diff(q, k, v, lam, lambda_init, *, gamma=None, eps=1e-5, causal=False, k_len=None, q_start=None, out=None):
@@ -1063,7 +1073,7 @@ def attn_diff(q, k, v, lam, lambda_init, *, gamma=None, eps=1e-5, causal=False, 
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return attn_diff(q, k, v, lam, lambda_init, gamma=gamma, eps=eps, causal=causal, k_len=k_len, q_start=q_start, out=out)
-    o = out if out is not None else torch.empty((B, n_q, H, 128), dtype=q.dtype, device=dev)
+    o = out if out is not None else q.new_empty((B, n_q, H, 128))
     if worklog is not None:
         _wl("attn_diff", 512.0 * B * H * n_q * n_k, 2.0 * 128 * B * (2 * H * n_q + 2 * KV * n_k))
     need = _lib.svd_attn_diff_ws_bytes(B, n_q, n_k, H, KV)
@@ -1071,5 +1081,5 @@ def attn_diff(q, k, v, lam, lambda_init, *, gamma=None, eps=1e-5, causal=False, 
     check(_lib.svd_attn_diff(q.data_ptr(), *_strides4(q), k.data_ptr(), *_strides4(k), v.data_ptr(), *_strides4(v), o.data_ptr(), *_strides4(o), lam.data_ptr(),
                              lambda_init, gamma.data_ptr() if gamma is not None else None, eps, k_len.data_ptr() if k_len is not None else None,
                              q_start.data_ptr() if q_start is not None else None, B, n_q, n_k, H, KV, int(causal), ws.data_ptr() if ws is not None else None,
-                             max(need, 0), _DT[q.dtype], torch.cuda.current_stream().cuda_stream), "svd_attn_diff")
+                             max(need, 0), _DT[q.dtype], _raw_stream(dev.index)), "svd_attn_diff")
     return o
