@@ -9,7 +9,9 @@
 //   O_i^T[channel][query] += V^T P_i^T  the accumulator registers 8 s .. 8 s + 7 of S_i^T are the B operand of step s as they stand, if the A operand holds
 //                                      the same keys in the same order: half h holds keys 16 s + 4 h + (0..3) and 16 s + 8 + 4 h + (0..3).
 // P is rounded to the 16-bit type for the matrix cores (at most half a step of the type relative to each weight); scores, maxima, sums and both accumulators
-// are fp32, and the row sums add the unrounded weights.
+// are fp32, and the row sums add the unrounded weights.  The maps' difference makes these roundings weigh more than the result's own (lambda 0.8, scores of
+// deviation 1: together 1.6 roundings of the result in the 2-norm), so what map 1's weights lose is rounded once more and multiplied as well: for all keys where the keys
+// and values are what takes the time (1.1 to 1.2 roundings), for 16 of 32 where the products are (1.45 at most; none, half, all of them: 727, 804, 896 us for 2 x 9216 tokens).
 // The heads of a group that share a key / value head are rows of one product: row r = query * group + head, so a causal tile of rows spans few queries.
 #include "svd_common.h"
 
@@ -78,10 +80,11 @@ __device__ __forceinline__ float halves_max(float v) {
 
 // Q_LDS: three of map 2's four query fragments wait in the wave's 3 KiB of LDS instead of 12 registers
 template <class E, bool Q_LDS = false> struct DiffWave {
+    static constexpr int RESTS = Q_LDS ? 1 : 2;          // 16-key halves of a step whose weights' rests are multiplied
     uint4 qf[8];
     uint4* q_lds;
     f32x16_t o[2][4], s[2];
-    uint32_t pk[2][8];
+    uint32_t pk[2][8], rest[4 * RESTS];        // weights in 16 bits; what map 1's lost
     float m[2], l[2];
     int l31, hi, seen, first;          // keys that this lane's query sees; the fewest that any query of the wave sees
     bool bad;                          // a value that is not finite in a tile with hidden places
@@ -162,9 +165,16 @@ template <class E, bool Q_LDS = false> struct DiffWave {
         const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i][2 * e], C_EXP, -m[i])), p1 = __builtin_amdgcn_exp2f(fmaf(s[i][2 * e + 1], C_EXP, -m[i]));
         l[i] += p0 + p1;
         pk[i][e] = E::pack(p0, p1);
+        if (i == 0 && e < 4 * RESTS) rest[e] = E::pack(fmaf(E::lo(pk[i][e]), -1.f, p0), fmaf(E::hi(pk[i][e]), -1.f, p1));
     }
     __device__ __forceinline__ uint4 p_frag(int i, int q) const { return make_uint4(pk[i][4 * q], pk[i][4 * q + 1], pk[i][4 * q + 2], pk[i][4 * q + 3]); }
-    __device__ __forceinline__ void values(int i, int q, int t, uint32_t sV) { o[i][t] = E::mfma(v_frag(((sV + va) ^ (t << 6)) + q * 16 * ROW_B), p_frag(i, q), o[i][t]); }
+    __device__ __forceinline__ uint4 r_frag(int q) const { return make_uint4(rest[4 * q], rest[4 * q + 1], rest[4 * q + 2], rest[4 * q + 3]); }
+    // o_i^T += V^T P_i^T for 16 keys and 32 channels
+    __device__ __forceinline__ void add(int i, int q, int t, uint4 vf) {
+        o[i][t] = E::mfma(vf, p_frag(i, q), o[i][t]);
+        if (i == 0 && q < RESTS) o[i][t] = E::mfma(vf, r_frag(q), o[i][t]);
+    }
+    __device__ __forceinline__ void values(int i, int q, int t, uint32_t sV) { add(i, q, t, v_frag(((sV + va) ^ (t << 6)) + q * 16 * ROW_B)); }
     __device__ __forceinline__ void look_for_bad(uint32_t sV) {
 #pragma unroll
         for (int q = 0; q < 2; ++q)
@@ -192,7 +202,7 @@ template <class E, bool Q_LDS = false> struct DiffWave {
                 for (int t = 0; t < 4; ++t) {
                     const uint4 vf = v_frag(((sV + va) ^ (t << 6)) + q * 16 * ROW_B);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) o[i][t] = E::mfma(vf, p_frag(i, q), o[i][t]);
+                    for (int i = 0; i < 2; ++i) add(i, q, t, vf);
                 }
         } else {
 #pragma unroll
@@ -211,7 +221,7 @@ template <class E, bool Q_LDS = false> struct DiffWave {
                     }
                     hit = E::mfma(NonFinite<E>::places(vf), make_uint4(see[0], see[1], see[2], see[3]), hit);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) o[i][t] = E::mfma(NonFinite<E>::cleared(vf), p_frag(i, q), o[i][t]);
+                    for (int i = 0; i < 2; ++i) add(i, q, t, NonFinite<E>::cleared(vf));
                 }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[0][t][r] = hit[r] > 0.f ? NAN : o[0][t][r];
@@ -226,23 +236,26 @@ template <class E, bool Q_LDS = false> struct DiffWave {
         auto kf = [&](int ks) { return k_frag((sK + ka) ^ ((4 * (1 - i) + ks) << 5)); };
         uint4 k[2], x[2], v[4];
         k[0] = kf(0); x[0] = q_frag(1 - i, 0);
-        v[0] = vf(0); v[1] = vf(1); v[2] = vf(2);
+        v[0] = vf(0); v[1] = vf(1);
         follow(i, top(i));
         // the four score products are a chain on one accumulator: they stand between the products with V, which go round four
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[1 - i][r] = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            if (e + 3 < 8) v[(e + 3) % 4] = vf(e + 3);
+            if (e + 2 < 8) v[(e + 2) % 4] = vf(e + 2);
             if (e % 2 == 0) {
                 if (e < 6) { k[(e / 2 + 1) & 1] = kf(e / 2 + 1); x[(e / 2 + 1) & 1] = q_frag(1 - i, e / 2 + 1); }
                 s[1 - i] = E::mfma(k[(e / 2) & 1], x[(e / 2) & 1], s[1 - i]);
             }
             o[1 - i][e & 3] = E::mfma(v[e % 4], p_frag(1 - i, e >> 2), o[1 - i][e & 3]);
+            if (1 - i == 0 && e > 0 && e <= 4 * RESTS) o[0][(e - 1) & 3] = E::mfma(v[(e - 1) % 4], r_frag((e - 1) >> 2), o[0][(e - 1) & 3]);          // a product later: not behind the same accumulator's
             weigh(i, e);
+            if (i == 0 && e < 4 * RESTS) asm volatile("" : "+v"(rest[e]));
             asm volatile("" : "+v"(pk[i][e]), "+v"(l[i]));          // made here, not where the next half needs it
-            __builtin_amdgcn_sched_barrier(0);                      // the reads stay where they are: three products (150 cycles) ahead of their use
+            __builtin_amdgcn_sched_barrier(0);                      // the reads stay where they are: two or three products ahead of their use
         }
+        if (1 - i == 0 && RESTS == 2) o[0][3] = E::mfma(v[7 % 4], r_frag(RESTS - 1), o[0][3]);
     }
     __device__ __forceinline__ void join_halves() {
 #pragma unroll
