@@ -398,13 +398,13 @@ int svd_rmsnorm(const void* X, int64_t ldx, const void* R, int64_t ldr, const fl
  *   X [M][ldx], W [N][ldw] row-major: both of in_dtype -- SVD_DTYPE_F16 | BF16 (== dtype), or SVD_DTYPE_F8 (e4m3, with optional row scales).
  *   bias [N] fp32 or NULL.  R [M][ldr] or NULL: 16-bit `dtype`, or fp32 with SVD_LIN_RES_F32 (R == Y with equal types and strides adds in place).
  *   Y [M][ldy]: 16-bit `dtype`, or fp32 with SVD_LIN_OUT_F32.  Y must not overlap X or W.
- *   Any M, N, K >= 1 (M == 0 returns SVD_OK), any alignment and leading dimensions; X and W rows that are 16-byte aligned with K * element size a multiple
- *   of 16, N and the leading dimensions of Y and R even and Y and R aligned to two elements, take the fast path.  (svd_gemm adds its residual before its
- *   activation; this entry adds it after.)
- *   ws: svd_linear_act_ws_bytes(...) bytes of scratch memory (16-byte aligned; may be NULL when that is 0), free again when the call's work on `stream` ends. */
+ *   Any M, N, K >= 1 (M == 0 returns SVD_OK), any alignment and leading dimensions of whole elements; K * element size < 2^23 for M > 64.
+ *   (svd_gemm adds its residual before its activation; this entry adds it after.)
+ *   ws: svd_linear_act_ws_bytes(...) bytes of scratch memory (16-byte aligned; may be NULL when that is 0), free again when the call's work on `stream` ends.
+ *   `aligned`: 1 if X, W, their leading dimensions and K are multiples of 16 bytes (and the dimensions under 2^23 bytes); 0 asks for room for copies that are. */
 enum { SVD_ACT_NONE = 0, SVD_ACT_RELU = 1, SVD_ACT_GELU = 2 /* erf */, SVD_ACT_GELU_TANH = 3, SVD_ACT_SILU = 4 };
 enum { SVD_LIN_RES_F32 = 1, SVD_LIN_OUT_F32 = 2 };
-int64_t svd_linear_act_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t flags, int32_t in_dtype);
+int64_t svd_linear_act_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t flags, int32_t in_dtype, int32_t aligned);
 int svd_linear_act(const void* X, int64_t ldx, const void* W, int64_t ldw, const float* xscale, const float* wscale, const float* bias,
                    const void* R, int64_t ldr, void* Y, int64_t ldy, int64_t M, int32_t N, int32_t K, int32_t act, int32_t flags,
                    void* ws, int64_t ws_bytes, int32_t in_dtype, int32_t dtype, svd_stream_t stream);

@@ -25,7 +25,7 @@ struct LinArgs {
     const float* xs; const float* ws; const float* bias;
     const void* R; int64_t ldr;
     void* Y; int64_t ldy;
-    int M, N, kbytes, act, res_f32, out_f32;
+    int M, N, kbytes, act, res_f32, out_f32, pair;          // pair: two adjacent columns of Y (and R) are one aligned access
 };
 
 // 64 bytes of K of 32 rows: lane l holds row l % 32.  Which k a lane's bytes are does not matter to a sum as long as both operands agree: half h of the wave holds
@@ -106,63 +106,6 @@ template <int EB> __device__ __forceinline__ uint4 load_chunk(const char* row, i
     return r;
 }
 
-// 128 x 128 outputs per workgroup of four waves (64 x 64 each); operands of any alignment, staged through registers.
-template <class In, class Eo> __global__ __launch_bounds__(256) void linear_any_kernel(LinArgs p, int tiles_n) {
-    __shared__ __attribute__((aligned(16))) char smem[2 * 128 * 128];
-    char* sA = smem; char* sB = smem + 128 * 128;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
-    const int m0 = (blockIdx.x / tiles_n) * 128, n0 = (blockIdx.x % tiles_n) * 128;
-    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    f32x16_t acc[2][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    for (int k0 = 0; k0 < p.kbytes; k0 += 128) {
-        uint4 ra[4], rb[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int row = j * 32 + (tid >> 3), ch = tid & 7;
-            ra[j] = load_chunk<In::kBytes>(p.X + (int64_t)min(m0 + row, p.M - 1) * p.ldx, k0 + ch * 16, p.kbytes);
-            rb[j] = load_chunk<In::kBytes>(p.W + (int64_t)min(n0 + row, p.N - 1) * p.ldw, k0 + ch * 16, p.kbytes);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int row = j * 32 + (tid >> 3), slot = (tid & 7) ^ ((row >> 1) & 7);
-            *(uint4*)(sA + row * 128 + slot * 16) = ra[j];
-            *(uint4*)(sB + row * 128 + slot * 16) = rb[j];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            Frag<In> a[2], b[2];
-            const int ch = 4 * s + 2 * hi;
-            auto chunk = [&](const char* base, int row, int c) { return *(const uint4*)(base + row * 128 + ((c ^ ((row >> 1) & 7)) << 4)); };
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                a[i].set(chunk(sA, wm + 32 * i + l31, ch), chunk(sA, wm + 32 * i + l31, ch + 1));
-                b[i].set(chunk(sB, wn + 32 * i + l31, ch), chunk(sB, wn + 32 * i + l31, ch + 1));
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = mma64<In>(a[i], b[j], acc[i][j]);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int m = m0 + wm + 32 * i + 8 * (r >> 2) + 4 * hi + (r & 3), n = n0 + wn + 32 * j + l31;
-                if (m < p.M && n < p.N) epilogue<Eo>(p, m, n, acc[i][j][r]);
-            }
-}
-
 // ---- large products: BM x BN outputs per workgroup of WM x WN waves, each TM x TN tiles of 32 x 32; rows 16-byte aligned ----
 // K goes in steps of 128 bytes (whole cache lines: with 64 the L2 has twice the requests to serve) through two LDS slots, rows of 128 bytes with 16-byte chunks
 // swizzled by (row >> 1) & 7: 16 lanes that read one chunk of 16 rows touch all 64 banks once.  A half step of 64 bytes multiplies fragments that the half before has read
@@ -170,6 +113,9 @@ template <class In, class Eo> __global__ __launch_bounds__(256) void linear_any_
 // step after the next: two halves of a step (2000 cycles of matrix work) ahead of its use, one barrier a step.
 // W's rows lie in LDS as even, then odd columns of each 64: a lane's two tiles of such a block are two adjacent columns, so results leave (and residuals come) as
 // pairs, 32 lanes a contiguous 128 (fp32: 256) bytes of a row.
+// Measured, 256 x 256: bf16 28800 x 1280 x 5120 onto an fp32 stream 392 us (0.96 PFLOP/s; two whole rounds 320 us, the split third 43, the join 17), e4m3
+// 28800 x 5120 x 1280 with GELU 258 us (1.46 PFLOP/s).  The same loop without its requests and LDS reads takes 232 of the 320 us (1.47 PFLOP/s, what a large library
+// product reaches), without either of them 286; of the 258 us the epilogue is about 90: one workgroup fills a CU, so nothing runs beside it.
 template <int WM_, int WN_, int TM_, int TN_> struct Tile {
     static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, WAVES = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32, SLOT = (BM + BN) * 128, REQ = (BM + BN) / 8 / WAVES;
 };
@@ -194,8 +140,8 @@ template <int ACT, int N> __device__ __forceinline__ void act_all(f32x16_t (&acc
 template <class Eo, int TM, int TN> __device__ __forceinline__ void finish_tiles(const LinArgs& p, f32x16_t (&acc)[TM * TN], int m0, int n0, const float* xs, bool whole, int l31, int hi) {
 #pragma unroll
     for (int b = 0; b < TN / 2; ++b) {
-        const int nc = min(n0 + 64 * b + 2 * l31, p.N - 2);
-        const float w0 = p.ws ? p.ws[nc] : 1.f, w1 = p.ws ? p.ws[nc + 1] : 1.f, b0 = p.bias ? p.bias[nc] : 0.f, b1 = p.bias ? p.bias[nc + 1] : 0.f;
+        const int c0 = min(n0 + 64 * b + 2 * l31, p.N - 1), c1 = min(c0 + 1, p.N - 1);
+        const float w0 = p.ws ? p.ws[c0] : 1.f, w1 = p.ws ? p.ws[c1] : 1.f, b0 = p.bias ? p.bias[c0] : 0.f, b1 = p.bias ? p.bias[c1] : 0.f;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -223,6 +169,22 @@ template <class Eo, int TM, int TN> __device__ __forceinline__ void finish_tiles
             const int n = n0 + 64 * b + 2 * l31, mb = m0 + 32 * i;
             f32x16_t &v0 = acc[i * TN + 2 * b], &v1 = acc[i * TN + 2 * b + 1];
             if (n >= p.N) continue;
+            if (!p.pair) {          // odd widths or strides: element by element
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int m = mb + 8 * (r >> 2) + (r & 3) + 4 * hi;
+                    if (m >= p.M) continue;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        if (n + c >= p.N) continue;
+                        float v = c ? v1[r] : v0[r];
+                        if (p.R) v += p.res_f32 ? ((const float*)p.R)[m * p.ldr + n + c] : Eo::to_f32(((const uint16_t*)p.R)[m * p.ldr + n + c]);
+                        if (p.out_f32) ((float*)p.Y)[m * p.ldy + n + c] = v;
+                        else ((uint16_t*)p.Y)[m * p.ldy + n + c] = Eo::from_f32(v);
+                    }
+                }
+                continue;
+            }
             if (p.R) {
                 const char* base = (const char*)p.R + ((int64_t)mb * p.ldr + n0 + 64 * b) * er;
                 const uint32_t lane_off = (4 * hi * (uint32_t)p.ldr + 2 * l31) * er;
@@ -253,6 +215,18 @@ template <class Eo, int TM, int TN> __device__ __forceinline__ void finish_tiles
                 }
             }
         }
+}
+
+// Rows of any alignment laid out anew, 16-byte aligned, zeros behind their end: a copy of X and W is cheap next to a product that needs tiles (the same tiles filled through
+// registers from unaligned rows: 543 us instead of 258 + 20 at 28800 x 5120 x 1280 e4m3).
+template <int EB> __global__ __launch_bounds__(256) void linear_align_kernel(const char* src, int64_t ld, char* dst, int64_t rows, int kbytes) {
+    const int chunks = (kbytes + 15) >> 4;
+    const int64_t n = rows * chunks;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / chunks;
+        const int c = (int)(i - row * chunks);
+        ((uint4*)dst)[i] = load_chunk<EB>(src + row * ld, c * 16, kbytes);
+    }
 }
 
 // Place of tile `w` of the list: 8 tiles of M by all tiles of N, then the next 8: the 32 workgroups that an XCD runs at once share 8 bands of X and 4 of W.
@@ -415,7 +389,8 @@ template <class Eo, class T> __global__ __launch_bounds__(T::WAVES * 64) void li
 }
 
 // ---- few rows: 32 columns x 32 TM rows per workgroup, its eight waves take 64-byte steps of K in turn and add up through LDS.  No staging: the weights are read
-// once, straight into fragments, and what bounds it is how many of their bytes are in flight; rows of any alignment. ----
+// once, straight into fragments, and what bounds it is latency and how many of their bytes are in flight; rows of any alignment.  One row of 1280 by 5120 columns, e4m3:
+// 5.0 us (6.6 MB, 1.3 TB/s); 77 x 1001 x 515 fp16: 11 us. ----
 template <class In, class Eo, int TM> __global__ __launch_bounds__(512) void linear_rows_kernel(LinArgs p, int tiles_n) {
     constexpr int NW = 8;
     __shared__ __attribute__((aligned(16))) float part[NW][TM * 16][64];
@@ -513,38 +488,52 @@ template <class In, class Eo, class T> int launch_tiles(const LinArgs& p, const 
     return SVD_OK;
 }
 
-template <class In, class Eo> int launch(const LinArgs& p, void* ws, int64_t ws_bytes, hipStream_t stream) {
+int64_t aligned_copy_bytes(int64_t M, int64_t N, int64_t kbytes) { return (M + N) * ((kbytes + 15) & ~15ll); }
+
+template <class In, class Eo> int launch(LinArgs p, void* ws, int64_t ws_bytes, hipStream_t stream) {
     const LinPlan plan = lin_plan(p.M, p.N, p.kbytes, In::kWiden);
-    if (ws_bytes < plan.ws || (plan.ws && !ws) || ((uintptr_t)ws & 15)) return SVD_EINVAL;
-    const uintptr_t pair = p.out_f32 ? (uintptr_t)p.Y & 7 : (uintptr_t)p.Y & 3, rpair = !p.R ? 0 : p.res_f32 ? (uintptr_t)p.R & 7 : (uintptr_t)p.R & 3;
-    const bool aligned = !(((uintptr_t)p.X | (uintptr_t)p.W | p.ldx | p.ldw | p.kbytes) & 15) && !pair && !rpair && !((p.ldy | (p.R ? p.ldr : 0) | p.N) & 1) &&
-                         p.ldx < (1 << 23) && p.ldw < (1 << 23) && p.ldy < (1 << 26) && p.ldr < (1 << 26);          // tiles are addressed with 32-bit offsets
     if (plan.form == ROWS) {
         const int tm = p.M <= 32 ? 1 : 2;
         const int64_t tn = (p.N + 31) / 32, grid = (p.M + 32 * tm - 1) / (32 * tm) * tn;
         if (grid > 0x7fffffff) return SVD_EINVAL;
         if (tm == 1) hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 1>), dim3((unsigned)grid), dim3(512), 0, stream, p, (int)tn);
         else hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 2>), dim3((unsigned)grid), dim3(512), 0, stream, p, (int)tn);
-    } else if (!aligned) {
-        const int64_t tn = (p.N + 127) / 128, grid = (int64_t)((p.M + 127) / 128) * tn;
-        if (grid > 0x7fffffff) return SVD_EINVAL;
-        hipLaunchKernelGGL((linear_any_kernel<In, Eo>), dim3((unsigned)grid), dim3(256), 0, stream, p, (int)tn);
-    } else {
-        if ((int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128) * 8 > 0x7fffffff) return SVD_EINVAL;
-        if constexpr (!In::kWiden)
-            if (plan.form == BIG) return launch_tiles<In, Eo, Big>(p, plan, (float*)ws, stream);
-        return launch_tiles<In, Eo, Small>(p, plan, (float*)ws, stream);
+        SVD_CHECK_LAUNCH("linear_act");
+        return SVD_OK;
     }
-    SVD_CHECK_LAUNCH("linear_act");
-    return SVD_OK;
+    constexpr int64_t FAR = 1 << 23;          // tiles are addressed with 32-bit offsets
+    const bool anew = (((uintptr_t)p.X | (uintptr_t)p.W | p.ldx | p.ldw | p.kbytes) & 15) || p.ldx >= FAR || p.ldw >= FAR;
+    if (ws_bytes < plan.ws + (anew ? aligned_copy_bytes(p.M, p.N, p.kbytes) : 0) || ((plan.ws || anew) && !ws) || ((uintptr_t)ws & 15)) return SVD_EINVAL;
+    if ((int64_t)((p.M + 127) / 128) * ((p.N + 127) / 128) * 8 > 0x7fffffff) return SVD_EINVAL;
+    if (anew) {
+        const int kp = (p.kbytes + 15) & ~15;
+        if (kp >= FAR) return SVD_EINVAL;
+        char *x = (char*)ws + plan.ws, *w = x + (int64_t)p.M * kp;
+        auto copy = [&](const char* src, int64_t ld, char* dst, int64_t rows) {
+            const int64_t blocks = (rows * (kp >> 4) + 255) / 256;
+            hipLaunchKernelGGL((linear_align_kernel<In::kBytes>), dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, stream, src, ld, dst, rows, p.kbytes);
+        };
+        copy(p.X, p.ldx, x, p.M);
+        SVD_CHECK_LAUNCH("linear_act");
+        copy(p.W, p.ldw, w, p.N);
+        SVD_CHECK_LAUNCH("linear_act");
+        p.X = x; p.W = w; p.ldx = p.ldw = p.kbytes = kp;
+    }
+    p.pair = !((p.out_f32 ? (uintptr_t)p.Y & 7 : (uintptr_t)p.Y & 3) | (!p.R ? 0 : p.res_f32 ? (uintptr_t)p.R & 7 : (uintptr_t)p.R & 3) | ((p.ldy | (p.R ? p.ldr : 0) | p.N) & 1)) &&
+             p.ldy < (1 << 26) && p.ldr < (1 << 26);
+    if constexpr (!In::kWiden)
+        if (plan.form == BIG) return launch_tiles<In, Eo, Big>(p, plan, (float*)ws, stream);
+    return launch_tiles<In, Eo, Small>(p, plan, (float*)ws, stream);
 }
 
 }  // namespace
 
-extern "C" int64_t svd_linear_act_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t flags, int32_t in_dtype) {
+extern "C" int64_t svd_linear_act_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t flags, int32_t in_dtype, int32_t aligned) {
     if (M < 0 || M > 0x7fffff00 || N < 1 || N > 0x7fffff00 || K < 1 || K > 0x3fffff00) return SVD_EINVAL;
     const bool f8 = in_dtype == SVD_DTYPE_F8;
-    return lin_plan(M, N, (int64_t)K * (f8 ? 1 : 2), f8 && (flags & SVD_LIN_OUT_F32)).ws;
+    const int64_t kbytes = (int64_t)K * (f8 ? 1 : 2);
+    const LinPlan plan = lin_plan(M, N, kbytes, f8 && (flags & SVD_LIN_OUT_F32));
+    return plan.ws + (plan.form != ROWS && !aligned ? aligned_copy_bytes(M, N, kbytes) : 0);
 }
 
 extern "C" int svd_linear_act(const void* X, int64_t ldx, const void* W, int64_t ldw, const float* xscale, const float* wscale, const float* bias,
@@ -561,7 +550,7 @@ extern "C" int svd_linear_act(const void* X, int64_t ldx, const void* W, int64_t
     if ((f4 & 3) || (f2 & 1)) return SVD_EINVAL;
     if (M == 0) return SVD_OK;
     const LinArgs p = {(const char*)X, ldx * es, (const char*)W, ldw * es, xscale, wscale, bias, R, ldr, Y, ldy, (int)M, N, K * es, act,
-                       !!(flags & SVD_LIN_RES_F32), !!(flags & SVD_LIN_OUT_F32)};
+                       !!(flags & SVD_LIN_RES_F32), !!(flags & SVD_LIN_OUT_F32), 0};
     if (in_dtype == SVD_DTYPE_F16) return launch<InF16, ElemF16>(p, ws, ws_bytes, (hipStream_t)stream);
     if (in_dtype == SVD_DTYPE_BF16) return launch<InBF16, ElemBF16>(p, ws, ws_bytes, (hipStream_t)stream);
     if (p.out_f32) return dtype == SVD_DTYPE_F16 ? launch<InF8Wide, ElemF16>(p, ws, ws_bytes, (hipStream_t)stream) : launch<InF8Wide, ElemBF16>(p, ws, ws_bytes, (hipStream_t)stream);

@@ -64,6 +64,8 @@ __global__ __launch_bounds__(256) void rmsnorm_row_kernel(const void* X, int64_t
 
 // Rows in registers: TPR threads to a row, 8 channels at a time, at most 5 pieces a thread; one read and one write of everything.  x and r are all requested before
 // the first is used (up to 240 bytes a thread in flight).  A row of 16 or 64 threads is reduced inside a wave, one of 256 through LDS.
+// What bounds it is memory: 115200 x 640, fp16 x onto an fp32 stream, e4m3 out: 152 us, 5.3 TB/s (a large copy: 5.1); 9217 x 1277 bf16 rows of odd width 26 us, 3.6 TB/s.
+// One row of 1280 takes 3.3 us, all of it latency.  (The one-row kernel's three passes: 604 and 43 us.)
 // AL: 16-byte aligned rows of whole pieces; else pieces of any alignment (the memory pipe takes them, at more lines per access) and a last one element by element.
 template <class E, bool F32, bool AL> __device__ __forceinline__ void load8(const void* row, int c, int n, float (&v)[8]) {
     constexpr int EB = F32 ? 4 : 2;

@@ -158,7 +158,7 @@ def _load():
     lib.svd_vfi_tta_average.argtypes = [vp, vp, vp, i32, i32, vp]
     lib.svd_rmsnorm.argtypes = [vp, i64, vp, i64, vp, f32, vp, i64, vp, vp, i64, i64, i32, i32, i32, vp]
     lib.svd_linear_act_ws_bytes.restype = C.c_int64
-    lib.svd_linear_act_ws_bytes.argtypes = [i64, i32, i32, i32, i32]
+    lib.svd_linear_act_ws_bytes.argtypes = [i64, i32, i32, i32, i32, i32]
     lib.svd_linear_act.argtypes = [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, i64, i64, i32, i32, i32, i32, vp, i64, i32, i32, vp]
     lib.svd_attn_diff_ws_bytes.restype = C.c_int64
     lib.svd_attn_diff_ws_bytes.argtypes = [i32] * 5

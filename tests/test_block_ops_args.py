@@ -46,13 +46,18 @@ def test_linear_refuses(lib, bad):
 
 def test_linear_scratch_size(lib):
     f = lib.svd_linear_act_ws_bytes
-    assert f(-1, 1, 1, 0, F16) == EINVAL and f(1, 0, 1, 0, F16) == EINVAL and f(1, 1, 0, 0, F16) == EINVAL
-    assert f(0, 64, 64, 0, F16) == 0 and f(1, 5120, 1280, 0, F8) == 0 and f(64, 64, 64, 0, F16) == 0
+    assert f(-1, 1, 1, 0, F16, 1) == EINVAL and f(1, 0, 1, 0, F16, 1) == EINVAL and f(1, 1, 0, 0, F16, 1) == EINVAL
+    assert f(0, 64, 64, 0, F16, 0) == 0 and f(1, 5120, 1280, 0, F8, 0) == 0 and f(64, 64, 64, 0, F16, 0) == 0
     for m, n, k, it, fl in [(28800, 1280, 5120, BF16, 0), (2304, 1280, 5120, F8, 0), (2304, 1280, 5120, F8, 2), (1100, 1040, 4096, F16, 0)]:
-        need = f(m, n, k, fl, it)
+        need = f(m, n, k, fl, it, 1)
         assert 0 < need <= 1 << 29 and need % 16 == 0
         big = dict(M=m, N=n, K=k, ldx=k, ldw=k, ldy=n, it=it, flags=fl, dt=BF16 if it != F16 else F16)
         assert linear(lib, **big) == EINVAL and linear(lib, scratch=A, sb=need - 1, **big) == EINVAL and linear(lib, scratch=A + 8, sb=need, **big) == EINVAL
+        copies = f(m, n, k, fl, it, 0)
+        assert copies == need + (m + n) * k * (1 if it == F8 else 2)
+        assert linear(lib, scratch=A, sb=copies - 1, **dict(big, ldx=k + 1)) == EINVAL          # unaligned rows need room for aligned copies
+    far = dict(M=1100, N=1040, K=1 << 23, ldx=1 << 23, ldw=1 << 23, ldy=1040)
+    assert linear(lib, scratch=A, sb=1 << 60, **far) == EINVAL                                  # rows that no tile can address
 
 
 def test_linear_no_rows(lib):

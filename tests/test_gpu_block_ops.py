@@ -241,7 +241,7 @@ def test_linear_picks_rows_and_columns(ops, t, m, n, k):
 
 
 @pytest.mark.parametrize("t", [BF16, F8], ids=str)
-@pytest.mark.parametrize("m,n,k", [(3, 320, 640), (90, 320, 640), (600, 328, 640)])
+@pytest.mark.parametrize("m,n,k", [(3, 320, 640), (90, 320, 640), (600, 328, 640), (1200, 1040, 640)])
 @pytest.mark.parametrize("off", [0, 16, 3])
 def test_linear_views_and_in_place_residual(ops, t, m, n, k, off):
     """Operands and destination are column ranges of wider rows; the destination is the residual; what surrounds it stays."""
