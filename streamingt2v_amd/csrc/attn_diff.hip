@@ -308,7 +308,7 @@ template <class E, bool Q_LDS = false> struct DiffWave {
 // does map 2's scores of step j and its products with V of step j - 1; while map 2's weights are made, map 1's scores of step j + 1 and its products with V of step j.
 // So K is read a step ahead and V a step behind: rings of four 8-KiB slots each, requests two steps ahead, one barrier a step.
 // 2 x 9216 tokens, 5 heads, fp16: 804 us (0.81 PFLOP/s of the one-pass work, 0.95 with the rests' products; 720 workgroups on 512 places leave the second round half
-// empty: at full rounds 0.93 and 1.08).  4 causal prompts of 1001 to 2001 tokens, 8 heads on 4: 104 us.
+// empty: at full rounds 0.93 and 1.08).  4 causal prompts of 1001 to 2001 tokens, 8 heads on 4: 84 us (104 with long rows first everywhere).
 template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kernel(DiffArgs p, int row_blocks) {
     constexpr int SLOT_B = 32 * ROW_B, RING_B = 4 * SLOT_B;          // K ring, then V ring
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -319,7 +319,10 @@ template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kern
         const int n = gridDim.x, x = blockIdx.x & 7, q = n >> 3, r = n & 7;
         wg = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (blockIdx.x >> 3);
     }
-    const int rb = row_blocks - 1 - wg % row_blocks, bh = wg / row_blocks, h = bh % p.kv_heads, b = bh / p.kv_heads;      // causal: the longest rows first
+    // Causal rows differ in length.  Where all workgroups are on the chip at once (two to a CU), every other head runs from the short rows to the long ones, so that the two
+    // of a CU are a long and a short one; else the long ones go first, for a short end.
+    const int bh = wg / row_blocks, u = wg % row_blocks, h = bh % p.kv_heads, b = bh / p.kv_heads;
+    const int rb = gridDim.x <= 512 && (bh & 1) ? u : row_blocks - 1 - u;
     const int rows = p.n_q * p.group, row0 = rb * 128 + wave * 32;
     const int rc = min(row0 + (lane & 31), rows - 1), q = rc / p.group, head = h * p.group + rc % p.group;
     const int len = key_count(p, b);
