@@ -11,7 +11,7 @@
 // P is rounded to the 16-bit type for the matrix cores (at most half a step of the type relative to each weight); scores, maxima, sums and both accumulators
 // are fp32, and the row sums add the unrounded weights.  The maps' difference makes these roundings weigh more than the result's own (lambda 0.8, scores of
 // deviation 1: together 1.6 roundings of the result in the 2-norm), so what map 1's weights lose is rounded once more and multiplied as well: for all keys where the keys
-// and values are what takes the time (1.1 to 1.2 roundings), for 16 of 32 where the products are (1.45 at most; none, half, all of them: 727, 804, 896 us for 2 x 9216 tokens).
+// and values are what takes the time (1.1 to 1.2 roundings), for 16 of 32 where the products are (1.45 at most; none, half, all of them: 727, 804, 896 us for 2 x 9216 tokens when it was measured).
 // The heads of a group that share a key / value head are rows of one product: row r = query * group + head, so a causal tile of rows spans few queries.
 #include "svd_common.h"
 
@@ -162,7 +162,9 @@ template <class E, bool Q_LDS = false> struct DiffWave {
     }
     // weights of scores 2 e and 2 e + 1
     __device__ __forceinline__ void weigh(int i, int e) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i][2 * e], C_EXP, -m[i])), p1 = __builtin_amdgcn_exp2f(fmaf(s[i][2 * e + 1], C_EXP, -m[i]));
+        weights(i, e, __builtin_amdgcn_exp2f(fmaf(s[i][2 * e], C_EXP, -m[i])), __builtin_amdgcn_exp2f(fmaf(s[i][2 * e + 1], C_EXP, -m[i])));
+    }
+    __device__ __forceinline__ void weights(int i, int e, float p0, float p1) {
         l[i] += p0 + p1;
         pk[i][e] = E::pack(p0, p1);
         if (i == 0 && e < 4 * RESTS) rest[e] = E::pack(fmaf(E::lo(pk[i][e]), -1.f, p0), fmaf(E::hi(pk[i][e]), -1.f, p1));
@@ -237,25 +239,33 @@ template <class E, bool Q_LDS = false> struct DiffWave {
         uint4 k[2], x[2], v[4];
         k[0] = kf(0); x[0] = q_frag(1 - i, 0);
         v[0] = vf(0); v[1] = vf(1);
-        follow(i, top(i));
-        // the four score products are a chain on one accumulator: they stand between the products with V, which go round four
+        const float mx = top(i);
+        k[1] = kf(1); x[1] = q_frag(1 - i, 1);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[1 - i][r] = 0.f;
+        s[1 - i] = E::mfma(k[0], x[0], s[1 - i]);
+        follow(i, mx);
+        // A matrix instruction keeps its unit for 32 cycles and the wave, if the next one follows at once, waiting as long: two of them stand around half of the vector
+        // instructions of two weights each.  The four score products are a chain on one accumulator and lie apart, and so do a product and its rest's.
+        auto score = [&](int ks) { s[1 - i] = E::mfma(k[ks & 1], x[ks & 1], s[1 - i]); };
+        constexpr int AT2[2] = {2, 5}, AT3[2] = {4, 6};          // where the third and fourth stand: map 1's half has the rests' products in between
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             if (e + 2 < 8) v[(e + 2) % 4] = vf(e + 2);
-            if (e % 2 == 0) {
-                if (e < 6) { k[(e / 2 + 1) & 1] = kf(e / 2 + 1); x[(e / 2 + 1) & 1] = q_frag(1 - i, e / 2 + 1); }
-                s[1 - i] = E::mfma(k[(e / 2) & 1], x[(e / 2) & 1], s[1 - i]);
-            }
+            if (e == 0) { k[0] = kf(2); x[0] = q_frag(1 - i, 2); }
+            if (e == 1) { k[1] = kf(3); x[1] = q_frag(1 - i, 3); }
             o[1 - i][e & 3] = E::mfma(v[e % 4], p_frag(1 - i, e >> 2), o[1 - i][e & 3]);
-            if (1 - i == 0 && e > 0 && e <= 4 * RESTS) o[0][(e - 1) & 3] = E::mfma(v[(e - 1) % 4], r_frag((e - 1) >> 2), o[0][(e - 1) & 3]);          // a product later: not behind the same accumulator's
-            weigh(i, e);
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[i][2 * e], C_EXP, -m[i])), t1 = fmaf(s[i][2 * e + 1], C_EXP, -m[i]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (e == 0) score(1);
+            if (e == AT2[i]) score(2);
+            if (e == AT3[i]) score(3);
+            if (1 - i == 0 && e > 0 && e <= 4 * RESTS) o[0][(e - 1) & 3] = E::mfma(v[(e - 1) % 4], r_frag((e - 1) >> 2), o[0][(e - 1) & 3]);
+            weights(i, e, p0, __builtin_amdgcn_exp2f(t1));
             if (i == 0 && e < 4 * RESTS) asm volatile("" : "+v"(rest[e]));
             asm volatile("" : "+v"(pk[i][e]), "+v"(l[i]));          // made here, not where the next half needs it
-            __builtin_amdgcn_sched_barrier(0);                      // the reads stay where they are: two or three products ahead of their use
+            __builtin_amdgcn_sched_barrier(0);                      // the reads stay where they are: two products ahead of their use
         }
-        if (1 - i == 0 && RESTS == 2) o[0][3] = E::mfma(v[7 % 4], r_frag(RESTS - 1), o[0][3]);
     }
     __device__ __forceinline__ void join_halves() {
 #pragma unroll
@@ -307,8 +317,9 @@ template <class E, bool Q_LDS = false> struct DiffWave {
 // matrix unit (24 instructions of 32 cycles), so the two have to run at once inside a wave.  The maps take turns: while map 1's weights of step j are made, the matrix unit
 // does map 2's scores of step j and its products with V of step j - 1; while map 2's weights are made, map 1's scores of step j + 1 and its products with V of step j.
 // So K is read a step ahead and V a step behind: rings of four 8-KiB slots each, requests two steps ahead, one barrier a step.
-// 2 x 9216 tokens, 5 heads, fp16: 804 us (0.81 PFLOP/s of the one-pass work, 0.95 with the rests' products; 720 workgroups on 512 places leave the second round half
-// empty: at full rounds 0.93 and 1.08).  4 causal prompts of 1001 to 2001 tokens, 8 heads on 4: 84 us (104 with long rows first everywhere).
+// 2 x 9216 tokens, 5 heads, fp16: 797 us (0.82 PFLOP/s of the one-pass work, 0.95 with the rests' products; the clock falls to 1.9 GHz under it; 720 workgroups on 512
+// places leave the second round half empty).  Before the maps took turns: 828 us without the rests.  4 causal prompts of 1001 to 2001 tokens, 8 heads on 4: 82 us (104
+// with long rows first everywhere).
 template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kernel(DiffArgs p, int row_blocks) {
     constexpr int SLOT_B = 32 * ROW_B, RING_B = 4 * SLOT_B;          // K ring, then V ring
     extern __shared__ __attribute__((aligned(16))) char smem[];
