@@ -387,9 +387,9 @@ int svd_vfi_tta_average(const float* pred2, float* out, uint8_t* out_u8, int32_t
  * RMS norm, optionally of a residual sum:  s = x + r;  y = s * gamma / sqrt(mean(s^2) + eps).   csrc/rmsnorm.hip
  *   X [rows][ldx]  16-bit `dtype`, or fp32 with SVD_RMS_X_F32.     R [rows][ldr] or NULL: 16-bit, or fp32 with SVD_RMS_R_F32.
  *   S [rows][lds] or NULL: the sum s, in R's type (needs R; S == R with lds == ldr updates the residual stream in place).
- *   Y [rows][ldy]  16-bit `dtype`; with SVD_RMS_OUT_F8 e4m3 values and yscale[rows] fp32: y = yscale[row] * Y[row], yscale = max |y| / 448 (0 for a row of
- *     zeros; NaN, with NaN values, for a row whose square sum is not finite in fp32).
- *   gamma [channels] fp32 or NULL (1).  Any channels >= 1, any alignment and leading dimension of whole elements.  rows == 0 returns SVD_OK. */
+ *   Y [rows][ldy]  16-bit `dtype`; with SVD_RMS_OUT_F8 e4m3 values and yscale[rows] fp32: y = yscale[row] * Y[row], yscale = max |y| / 448, at least
+ *     2^-126 (0 for a row of zeros; NaN, with NaN values, for a row whose square sum is not finite in fp32).
+ *   gamma [channels] fp32 or NULL (1).  Any channels from 1 to 2^31 - 256, any alignment and leading dimension of whole elements.  rows == 0 returns SVD_OK. */
 enum { SVD_RMS_X_F32 = 1, SVD_RMS_R_F32 = 2, SVD_RMS_OUT_F8 = 4 };
 int svd_rmsnorm(const void* X, int64_t ldx, const void* R, int64_t ldr, const float* gamma, float eps, void* Y, int64_t ldy, float* yscale,
                 void* S, int64_t lds, int64_t rows, int32_t channels, int32_t flags, int32_t dtype, svd_stream_t stream);
@@ -398,7 +398,7 @@ int svd_rmsnorm(const void* X, int64_t ldx, const void* R, int64_t ldr, const fl
  *   X [M][ldx], W [N][ldw] row-major: both of in_dtype -- SVD_DTYPE_F16 | BF16 (== dtype), or SVD_DTYPE_F8 (e4m3, with optional row scales).
  *   bias [N] fp32 or NULL.  R [M][ldr] or NULL: 16-bit `dtype`, or fp32 with SVD_LIN_RES_F32 (R == Y with equal types and strides adds in place).
  *   Y [M][ldy]: 16-bit `dtype`, or fp32 with SVD_LIN_OUT_F32.  Y must not overlap X or W.
- *   Any M, N, K >= 1 (M == 0 returns SVD_OK), any alignment and leading dimensions of whole elements; K * element size < 2^23 for M > 64.
+ *   Any M, N, K >= 1 (M == 0 returns SVD_OK), any alignment and leading dimensions of whole elements; K * element size < 2^23 for M > 64; K < 2^30 - 4096.
  *   (svd_gemm adds its residual before its activation; this entry adds it after.)
  *   ws: svd_linear_act_ws_bytes(...) bytes of scratch memory (16-byte aligned; may be NULL when that is 0), free again when the call's work on `stream` ends.
  *   `aligned`: 1 if X, W, their leading dimensions and K are multiples of 16 bytes (and the dimensions under 2^23 bytes); 0 asks for room for copies that are. */

@@ -38,6 +38,12 @@ __device__ __forceinline__ float diff_lambda(const float* lam, float lambda_init
     return expf(d1) - expf(d2) + lambda_init;
 }
 
+// the factor of the head's norm; zeros stay zeros with eps = 0 too
+__device__ __forceinline__ float diff_norm(float square_sum, const DiffArgs& p) {
+    const float d = square_sum * (1.f / 128.f) + p.eps;
+    return d == 0.f ? 0.f : (1.f - p.lambda_init) / sqrtf(d);
+}
+
 // keys of sequence b, in [0, n_k] whatever the lengths' tensor holds
 __device__ __forceinline__ int key_count(const DiffArgs& p, int b) { return p.k_len ? max(0, min(p.k_len[b], p.n_k)) : p.n_k; }
 // number of keys query q sees
@@ -69,6 +75,7 @@ template <class E> struct NonFinite {
 //   K: slot ^ (key & 15): 16 lanes that read one slot of 16 different keys (ds_read_b128, A operand: lane = key) touch all 64 banks once;
 //   V: slot ^ (4 (key & 3)): a transposing read takes 4 keys x 16 channels per 16 lanes; 32 lanes touch 4 keys x 2 x 32 bytes, all 64 banks once.
 constexpr int ROW_B = 256;
+constexpr int Q_B = 3 * 64 * 16;          // three query fragments of a wave
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
@@ -286,7 +293,7 @@ template <class E, bool Q_LDS = false> struct DiffWave {
                 ss = fmaf(o[0][t][r], o[0][t][r], ss);
             }
         ss += __shfl_xor(ss, 32, 64);
-        const float norm = p.gamma ? (1.f - p.lambda_init) / sqrtf(ss * (1.f / 128.f) + p.eps) : 1.f;
+        const float norm = p.gamma ? diff_norm(ss, p) : 1.f;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -340,7 +347,7 @@ template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kern
     const int last = seen_by(p, b, len, min(rows - 1, rb * 128 + 127) / p.group);                 // the workgroup's last row sees the most keys
     const int mine = row0 < rows ? seen_by(p, b, len, min(rows - 1, row0 + 31) / p.group) : 0;    // ... and the wave's
     DiffWave<E, true> w;
-    w.init(p.Q + b * p.q_sb + q * p.q_st + head * p.q_sh, lane, (uint4*)(smem + 2 * RING_B + wave * 3072));
+    w.init(p.Q + b * p.q_sb + q * p.q_st + head * p.q_sh, lane, (uint4*)(smem + 2 * RING_B + wave * Q_B));
     w.seen = seen_by(p, b, len, q);
     w.first = seen_by(p, b, len, min(rows - 1, row0) / p.group);
     const svd_bf16* Kb = p.K + b * p.k_sb + h * p.k_sh;
@@ -537,7 +544,7 @@ template <class E> __global__ __launch_bounds__(256) void attn_diff_join_kernel(
     const float w0 = l[0] == 0.f ? 0.f : 1.f / l[0], w1 = l[1] == 0.f ? 0.f : lam / l[1];
     float y0 = o[0][0] * w0 - o[1][0] * w1, y1 = o[0][1] * w0 - o[1][1] * w1;
     if (p.gamma) {
-        const float norm = (1.f - p.lambda_init) / sqrtf(wave_sum(fmaf(y0, y0, y1 * y1)) * (1.f / 128.f) + p.eps);
+        const float norm = diff_norm(wave_sum(fmaf(y0, y0, y1 * y1)), p);
         y0 *= norm * p.gamma[2 * lane]; y1 *= norm * p.gamma[2 * lane + 1];
     }
     *(uint32_t*)(p.O + b * p.o_sb + (row / p.group) * p.o_st + (h * p.group + row % p.group) * p.o_sh + 2 * lane) = E::pack(y0, y1);
@@ -581,13 +588,14 @@ extern "C" int svd_attn_diff(const svd_bf16* Q, int64_t q_sb, int64_t q_st, int6
     if (((uintptr_t)Q | (uintptr_t)K | (uintptr_t)V | (uintptr_t)O) & 15 || ((uintptr_t)lam | (uintptr_t)gamma | (uintptr_t)k_len | (uintptr_t)q_start) & 3) return SVD_EINVAL;
     if (k_st < 0 || v_st < 0 || k_st > (1 << 25) || v_st > (1 << 25)) return SVD_EINVAL;          // a tile's rows are addressed with 32-bit offsets
     const int group = heads / kv_heads;
-    if ((int64_t)n_q * group > 0x7fffff00 || n_k > 0x7fffff00) return SVD_EINVAL;
+    // positions are 32-bit numbers, and the last shares of a wave's keys may begin and end up to 1024 tiles behind the last key
+    if ((int64_t)n_q * group > 0x7fffff00 || n_k > 0x7fff0000) return SVD_EINVAL;
     const DiffArgs p = {Q, q_sb, q_st, q_sh, K, k_sb, k_st, k_sh, V, v_sb, v_st, v_sh, O, o_sb, o_st, o_sh, lam, lambda_init, gamma, eps, k_len, q_start,
                         n_q, n_k, kv_heads, group, causal};
     const int64_t grid = (int64_t)plan.row_blocks * batch * kv_heads * plan.shares;
     if (grid > 0x7fffffff || (int64_t)batch * heads * n_q > 0x7fffffff) return SVD_EINVAL;
     if (!plan.waves) {
-        constexpr int LDS = 8 * 32 * ROW_B + 4 * 3072;          // rings and map 2's queries: 76 KiB, two workgroups on a CU (two of 80 do not fit)
+        constexpr int LDS = 8 * 32 * ROW_B + 4 * Q_B;          // rings and map 2's queries: 76 KiB, two workgroups on a CU (two of 80 do not fit)
         SVD_DISPATCH_DTYPE(dtype, {
             SVD_ALLOW_LDS(attn_diff_rows_kernel<E>, LDS);
             hipLaunchKernelGGL((attn_diff_rows_kernel<E>), dim3((unsigned)grid), dim3(256), LDS, (hipStream_t)stream, p, plan.row_blocks);

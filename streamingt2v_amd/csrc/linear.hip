@@ -529,7 +529,7 @@ template <class In, class Eo> int launch(LinArgs p, void* ws, int64_t ws_bytes, 
 }  // namespace
 
 extern "C" int64_t svd_linear_act_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t flags, int32_t in_dtype, int32_t aligned) {
-    if (M < 0 || M > 0x7fffff00 || N < 1 || N > 0x7fffff00 || K < 1 || K > 0x3fffff00) return SVD_EINVAL;
+    if (M < 0 || M > 0x7fffff00 || N < 1 || N > 0x7fffff00 || K < 1 || K > 0x3fffefff) return SVD_EINVAL;
     const bool f8 = in_dtype == SVD_DTYPE_F8;
     const int64_t kbytes = (int64_t)K * (f8 ? 1 : 2);
     const LinPlan plan = lin_plan(M, N, kbytes, f8 && (flags & SVD_LIN_OUT_F32));
@@ -540,7 +540,7 @@ extern "C" int svd_linear_act(const void* X, int64_t ldx, const void* W, int64_t
                               const void* R, int64_t ldr, void* Y, int64_t ldy, int64_t M, int32_t N, int32_t K, int32_t act, int32_t flags,
                               void* ws, int64_t ws_bytes, int32_t in_dtype, int32_t dtype, svd_stream_t stream) {
     const int es = in_dtype == SVD_DTYPE_F8 ? 1 : 2;
-    if (!X || !W || !Y || M < 0 || M > 0x7fffff00 || N < 1 || N > 0x7fffff00 || K < 1 || K > 0x3fffff00 || ldx < K || ldw < K || ldy < N || (R && ldr < N)) return SVD_EINVAL;
+    if (!X || !W || !Y || M < 0 || M > 0x7fffff00 || N < 1 || N > 0x7fffff00 || K < 1 || K > 0x3fffefff || ldx < K || ldw < K || ldy < N || (R && ldr < N)) return SVD_EINVAL;
     if (act < SVD_ACT_NONE || act > SVD_ACT_SILU || (flags & ~(SVD_LIN_RES_F32 | SVD_LIN_OUT_F32)) || (!R && (flags & SVD_LIN_RES_F32))) return SVD_EINVAL;
     if (dtype != SVD_DTYPE_BF16 && dtype != SVD_DTYPE_F16) return SVD_EINVAL;
     if (in_dtype != SVD_DTYPE_F8 && in_dtype != dtype) return SVD_EINVAL;

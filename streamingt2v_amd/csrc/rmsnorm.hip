@@ -9,7 +9,10 @@ constexpr float F8_MAX = 448.f;              // largest finite e4m3
 
 // The row's scale.  A row of zeros has scale 0 and values 0; a row whose square sum is not finite (an Inf or NaN in it, or |s| beyond 1e19) has scale NaN
 // and values NaN, so that it cannot pass for numbers.  |y * inv| <= 448 (1 + 2^-22) rounds to at most 448: no clamp (which would swallow a NaN).
-__device__ __forceinline__ float f8_scale(float row_max, float square_sum) { return square_sum < INFINITY ? row_max / F8_MAX : NAN; }
+// The scale of any other row is at least 2^-126: 1 / a of a smaller one would be infinite.
+__device__ __forceinline__ float f8_scale(float row_max, float square_sum) {
+    return !(square_sum < INFINITY) ? NAN : row_max == 0.f ? 0.f : fmaxf(row_max / F8_MAX, 0x1p-126f);
+}
 __device__ __forceinline__ float f8_inv(float a) { return a == 0.f ? 0.f : 1.f / a; }
 
 // Rows wider than 10240 channels, and fp32 x with a 16-bit residual.  One workgroup per row, any width: three passes over the row (square sum, maximum, result); the second and third read from the L2.
@@ -213,12 +216,14 @@ template <class E, bool X32, int RM, bool F8, int TPR> void launch_vec(const Nor
     if (al) hipLaunchKernelGGL((rmsnorm_vec_kernel<E, X32, RM, F8, TPR, true>), grid, dim3(256), 0, n.stream, n.X, n.ldx, n.R, n.ldr, n.gamma, n.eps, n.Y, n.ldy, n.yscale, n.S, n.lds, n.rows, n.channels);
     else hipLaunchKernelGGL((rmsnorm_vec_kernel<E, X32, RM, F8, TPR, false>), grid, dim3(256), 0, n.stream, n.X, n.ldx, n.R, n.ldr, n.gamma, n.eps, n.Y, n.ldy, n.yscale, n.S, n.lds, n.rows, n.channels);
 }
-// Threads to a row from its width alone: five pieces a thread at most.  Wider rows, and fp32 x with a 16-bit residual, take the one-row kernel.
+// Threads to a row from its width alone: five pieces a thread at most.  Wider rows, and fp32 x with a 16-bit residual, take the one-row kernel; so do rows whose threads
+// would be 2^32 or more, which a launch cannot have.
 template <class E, bool X32, int RM, bool F8> bool try_vec(const NormCall& n, bool al) {
-    if (n.channels <= 640) launch_vec<E, X32, RM, F8, 16>(n, al);
-    else if (n.channels <= 2560) launch_vec<E, X32, RM, F8, 64>(n, al);
-    else if (n.channels <= 10240) launch_vec<E, X32, RM, F8, 256>(n, al);
-    else return false;
+    const int tpr = n.channels <= 640 ? 16 : n.channels <= 2560 ? 64 : 256;
+    if (n.channels > 10240 || n.rows > 0xffffff00ll / tpr) return false;
+    if (tpr == 16) launch_vec<E, X32, RM, F8, 16>(n, al);
+    else if (tpr == 64) launch_vec<E, X32, RM, F8, 64>(n, al);
+    else launch_vec<E, X32, RM, F8, 256>(n, al);
     return true;
 }
 template <class E, bool F8> bool try_all(const NormCall& n, bool x32, bool r32, bool al) {
@@ -232,21 +237,19 @@ template <class E, bool F8> bool try_all(const NormCall& n, bool x32, bool r32, 
 extern "C" int svd_rmsnorm(const void* X, int64_t ldx, const void* R, int64_t ldr, const float* gamma, float eps, void* Y, int64_t ldy, float* yscale,
                            void* S, int64_t lds, int64_t rows, int32_t channels, int32_t flags, int32_t dtype, svd_stream_t stream) {
     const bool x32 = flags & SVD_RMS_X_F32, r32 = flags & SVD_RMS_R_F32, f8 = flags & SVD_RMS_OUT_F8;
-    if (!X || !Y || rows < 0 || channels < 1 || ldx < channels || ldy < channels || (flags & ~7) || !(eps >= 0.f)) return SVD_EINVAL;
+    if (!X || !Y || rows < 0 || channels < 1 || channels > 0x7fffff00 || ldx < channels || ldy < channels || (flags & ~7) || !(eps >= 0.f)) return SVD_EINVAL;
     if ((R && ldr < channels) || (S && (!R || lds < channels)) || (!R && r32) || (f8 && !yscale)) return SVD_EINVAL;
     if (((uintptr_t)X & (x32 ? 3 : 1)) || ((uintptr_t)R & (r32 ? 3 : 1)) || ((uintptr_t)S & (r32 ? 3 : 1)) || (!f8 && ((uintptr_t)Y & 1)) || ((uintptr_t)gamma & 3) || ((uintptr_t)yscale & 3)) return SVD_EINVAL;
     if (dtype != SVD_DTYPE_BF16 && dtype != SVD_DTYPE_F16) return SVD_EINVAL;
     if (rows == 0) return SVD_OK;
-    if (rows < 0x7fffffff) {
-        const NormCall n = {X, ldx, R, ldr, gamma, eps, Y, ldy, yscale, S, lds, rows, channels, (hipStream_t)stream};
-        const int64_t by = (ldx * (x32 ? 4 : 2)) | (R ? ldr * (r32 ? 4 : 2) : 0) | (S ? lds * (r32 ? 4 : 2) : 0) | ldy * 2;          // (e4m3 pieces of 8 bytes: ldy * 2 a multiple of 16)
-        const bool al = !(channels & 7) && !(by & 15) && !(((uintptr_t)X | (uintptr_t)R | (uintptr_t)S | (uintptr_t)gamma) & 15) && !((uintptr_t)Y & (f8 ? 7 : 15));
-        bool done = false;
-        SVD_DISPATCH_DTYPE(dtype, done = f8 ? try_all<E, true>(n, x32, r32, al) : try_all<E, false>(n, x32, r32, al));
-        if (done) {
-            SVD_CHECK_LAUNCH("rmsnorm");
-            return SVD_OK;
-        }
+    const NormCall n = {X, ldx, R, ldr, gamma, eps, Y, ldy, yscale, S, lds, rows, channels, (hipStream_t)stream};
+    const int64_t by = (ldx * (x32 ? 4 : 2)) | (R ? ldr * (r32 ? 4 : 2) : 0) | (S ? lds * (r32 ? 4 : 2) : 0) | ldy * 2;          // (e4m3 pieces of 8 bytes: ldy * 2 a multiple of 16)
+    const bool al = !(channels & 7) && !(by & 15) && !(((uintptr_t)X | (uintptr_t)R | (uintptr_t)S | (uintptr_t)gamma) & 15) && !((uintptr_t)Y & (f8 ? 7 : 15));
+    bool done = false;
+    SVD_DISPATCH_DTYPE(dtype, done = f8 ? try_all<E, true>(n, x32, r32, al) : try_all<E, false>(n, x32, r32, al));
+    if (done) {
+        SVD_CHECK_LAUNCH("rmsnorm");
+        return SVD_OK;
     }
     const unsigned grid = (unsigned)(rows < 65536 ? rows : 65536);
 #define LAUNCH(X32, R32, F8) hipLaunchKernelGGL((rmsnorm_row_kernel<E, X32, R32, F8>), dim3(grid), dim3(256), 0, (hipStream_t)stream, X, ldx, R, ldr, gamma, eps, Y, ldy, yscale, S, lds, rows, channels)

@@ -1037,10 +1037,10 @@ def linear_act(x, w, *, bias=None, act=None, residual=None, x_scale=None, w_scal
         if M > 64:
             es = 1 if f8 else 2
             need = _lib.svd_linear_act_ws_bytes(M, N, K, flags, it, not ((x_ptr | w_ptr | ldx * es | ldw * es | K * es) & 15) and max(ldx, ldw) * es < 1 << 23)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None          # from the allocator, per call: its stream and its graph's pool own it
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None          # from the allocator, per call: its stream and its graph's pool own it
         check(_lib.svd_linear_act(x_ptr, ldx, w_ptr, ldw, x_scale.data_ptr() if x_scale is not None else None,
                                   w_scale.data_ptr() if w_scale is not None else None, bias.data_ptr() if bias is not None else None, r_ptr, ldr, y.data_ptr(),
-                                  _ld(y), M, N, K, _l.ACT[act], flags, ws.data_ptr() if need else None, need, it, _DT[e], _raw_stream(dev.index)), "svd_linear_act")
+                                  _ld(y), M, N, K, _l.ACT[act], flags, ws.data_ptr() if ws is not None else None, max(need, 0), it, _DT[e], _raw_stream(dev.index)), "svd_linear_act")
     return y
 
 

@@ -92,6 +92,17 @@ def test_attn_scratch_size(lib):
             assert attn(lib, B=B, nq=nq, nk=nk, H=H, KV=KV, wsb=n - 1) == EINVAL and attn(lib, B=B, nq=nq, nk=nk, H=H, KV=KV, ws=None, wsb=n) == EINVAL
 
 
+def test_sizes_that_32_bit_positions_cannot_walk(lib):
+    """The kernels step over channels, bytes of K and keys in 32-bit numbers; sizes whose last step would pass 2^31 are refused."""
+    big = 2 ** 31 - 1
+    for ch in (big, big - 254):
+        assert norm(lib, ch=ch, ldx=big, ldy=big) == EINVAL
+    for k in (2 ** 30 - 257, 2 ** 30 - 4096):
+        assert linear(lib, K=k, ldx=big, ldw=big) == EINVAL and lib.svd_linear_act_ws_bytes(4, 32, k, 0, F16, 1) == EINVAL
+    for n in (big, big - 255, 0x7fff0001):
+        assert attn(lib, nk=n, ks=(0, 0, 0), vs=(0, 0, 0)) == EINVAL
+
+
 def test_launchers_refuse_host_tensors():
     """There is no CPU form: the launchers say so instead of handing host addresses to a kernel."""
     from streamingt2v_amd import ops

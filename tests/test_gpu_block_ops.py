@@ -135,12 +135,39 @@ def test_rmsnorm_special_rows(ops):
     check_norm("rmsnorm special", y[3:], x[3:], None, None, 1e-6, False)
 
 
+@pytest.mark.parametrize("xt", [F32, BF16], ids=str)
+@pytest.mark.parametrize("ch", [64, 1277, 12000])
+def test_rmsnorm_tiny_rows_in_8_bits(ops, xt, ch):
+    """Rows so small that max |y| / 448 is below the smallest normal number: the scale stops there, and the values are numbers.
+    |scale q - y| <= (2^-4 + 5e-6) |y| + 2^-10 scale, as for any row; y's own rounding below 2^-126 is 2^-150, far below 2^-10 2^-126."""
+    randn = gen(23)
+    x = torch.cat([randn(2, ch) * s for s in (1e-30, 1e-36, 1e-38, 1e-39)]).to(xt)
+    gamma = 1 + randn(ch, scale=0.1)
+    q, a = ops.rmsnorm(x, gamma, eps=1e-6, f8=True)
+    _, y = norm64(x, None, gamma, 1e-6)
+    a64 = (y.abs().amax(1) / 448).clamp_min(2.0 ** -126)
+    within("rmsnorm tiny rows: scale", a, a64, (3e-6 + 2 * U32) * a64)
+    within("rmsnorm tiny rows: values", q.double() * a.double()[:, None], y, (2.0 ** -4 + 5e-6) * y.abs() + 2.0 ** -10 * a64[:, None])
+
+
 def test_rmsnorm_empty_and_many_rows(ops):
     assert ops.rmsnorm(torch.empty(0, 640, dtype=F16, device="cuda")).shape == (0, 640)
     q, a, s = ops.rmsnorm(torch.empty(0, 640, dtype=F16, device="cuda"), residual=torch.empty(0, 640, dtype=F32, device="cuda"), f8=True)
     assert q.shape == (0, 640) and a.shape == (0,) and s.dtype == F32
     x = gen(10)(70001, 24).to(BF16)
     check_norm("rmsnorm 70001 rows", ops.rmsnorm(x, None), x, None, None, 1e-6, False)
+
+
+def test_rmsnorm_more_threads_than_a_launch_has(ops):
+    """2^28 rows of 16 threads each would be 2^32: another form takes them."""
+    rows = (1 << 28) + 5
+    x = torch.empty(rows, 8, dtype=F16, device="cuda")
+    at = [slice(0, 1000), slice(rows // 2, rows // 2 + 1000), slice(rows - 1000, rows)]
+    for i, a in enumerate(at):
+        x[a] = gen(40 + i)(1000, 8).to(F16)
+    y = ops.rmsnorm(x, None)
+    for a in at:
+        check_norm("rmsnorm 2^28 rows", y[a], x[a], None, None, 1e-6, False)
 
 
 # ---------------------------------------------------------------------------------------------------------- linear_act
@@ -425,6 +452,21 @@ def test_attn_large_and_equal_scores(ops):
                     ("one key", randn(B, n_k, H, 128) * (torch.arange(n_k, device="cuda") == 700)[None, :, None, None] * 12)):
         for t in (F16, BF16):
             run_attn(ops, "attn scores " + name, q.to(t), k.to(t), v.to(t), 6, norm=False)
+
+
+@pytest.mark.parametrize("B,n_q,n_k,H,KV", [(3, 1, 600, 4, 2), (3, 3, 20, 4, 2), (80, 70, 90, 4, 2)])
+def test_attn_zeros_stay_zeros_without_eps(ops, B, n_q, n_k, H, KV):
+    """eps = 0: neither a query that sees no key nor one that sees only values of zero divides by zero; the others are as ever."""
+    randn = gen(60)
+    q, k, v = randn(B, n_q, H, 128).to(F16), randn(B, n_k, KV, 128).to(F16), randn(B, n_k, KV, 128).to(F16)
+    v[1] = 0
+    lens = torch.full((B,), n_k, dtype=torch.int32, device="cuda")
+    lens[0] = 0
+    lam, gamma = randn(4, 64, scale=0.1), 1 + randn(128, scale=0.1)
+    got = ops.attn_diff(q, k, v, lam, 0.4, gamma=gamma, eps=0.0, k_len=lens)
+    assert got[:2].eq(0).all()
+    near = ops.attn_diff(q, k, v, lam, 0.4, gamma=gamma, eps=1e-12, k_len=lens)
+    assert got[2:].ne(0).any() and torch.allclose(got[2:].float(), near[2:].float(), rtol=2.0 ** -9, atol=2.0 ** -24)          # a step of the type
 
 
 def test_attn_empty(ops):
