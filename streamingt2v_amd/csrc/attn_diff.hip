@@ -496,14 +496,41 @@ template <class E> __global__ __launch_bounds__(64, 2) void attn_diff_wave_kerne
     if (w.hi == 0) *(float4*)(part + 256) = make_float4(w.m[0], w.l[0], w.m[1], w.l[1]);
 }
 
+// Shares of a row's keys, joined one after the other: a lane holds two channels.
+__device__ __forceinline__ float2 gamma_pair(const DiffArgs& p, int lane) { return p.gamma ? make_float2(p.gamma[2 * lane], p.gamma[2 * lane + 1]) : make_float2(1.f, 1.f); }
+template <class E> struct Joined {
+    float m[2] = {M_NONE, M_NONE}, l[2] = {0.f, 0.f}, o[2][2] = {};
+    __device__ __forceinline__ void add(float4 ml, float2 x, float2 y) {          // maximum and sum of each map; the channels of each map's accumulator
+        const float m0 = fmaxf(m[0], ml.x), m1 = fmaxf(m[1], ml.z);
+        const float a0 = __builtin_amdgcn_exp2f(m[0] - m0), a1 = __builtin_amdgcn_exp2f(m[1] - m1), b0 = __builtin_amdgcn_exp2f(ml.x - m0), b1 = __builtin_amdgcn_exp2f(ml.z - m1);
+        m[0] = m0; m[1] = m1;
+        l[0] = fmaf(l[0], a0, ml.y * b0); l[1] = fmaf(l[1], a1, ml.w * b1);
+        o[0][0] = fmaf(o[0][0], a0, x.x * b0); o[0][1] = fmaf(o[0][1], a0, x.y * b0);
+        o[1][0] = fmaf(o[1][0], a1, y.x * b1); o[1][1] = fmaf(o[1][1], a1, y.y * b1);
+    }
+    // lam: diff_lambda, g: the lane's two channels of gamma, both requested before the wait for the shares
+    __device__ __forceinline__ void finish(const DiffArgs& p, int b, int h, int row, int lane, float lam, float2 g) const {
+        const float w0 = l[0] == 0.f ? 0.f : 1.f / l[0], w1 = l[1] == 0.f ? 0.f : lam / l[1];
+        float y0 = o[0][0] * w0 - o[1][0] * w1, y1 = o[0][1] * w0 - o[1][1] * w1;
+        if (p.gamma) {
+            const float norm = diff_norm(wave_sum(fmaf(y0, y0, y1 * y1)), p);
+            y0 *= norm * g.x; y1 *= norm * g.y;
+        }
+        *(uint32_t*)(p.O + b * p.o_sb + (row / p.group) * p.o_st + (h * p.group + row % p.group) * p.o_sh + 2 * lane) = E::pack(y0, y1);
+    }
+};
+
 // One workgroup per row: lane = two channels, the four waves take the shares in turn, four requested at once, and meet in LDS.  The order of the sums is fixed, so the result
 // does not depend on which share finished first.  (One wave and one share at a time: 11.6 us for 128 rows of 32 shares, 7.8 for 8 of 17.)
 template <class E> __global__ __launch_bounds__(256) void attn_diff_join_kernel(DiffArgs p, int shares, const float* ws) {
-    __shared__ float s_m[4][2], s_l[4][2], s_o[4][4][64];
+    __shared__ float4 s_ml[4];
+    __shared__ float2 s_o[4][2][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int rows = p.n_q * p.group, row = blockIdx.x % rows, bh = blockIdx.x / rows, h = bh % p.kv_heads, b = bh / p.kv_heads;
     const float* part = ws + (int64_t)blockIdx.x * shares * PART;
-    float m[2] = {M_NONE, M_NONE}, l[2] = {0.f, 0.f}, o[2][2] = {};
+    const float lam = diff_lambda(p.lam, p.lambda_init, lane);
+    const float2 g = gamma_pair(p, lane);
+    Joined<E> sum;
     for (int s0 = wave; s0 < shares; s0 += 16) {
         float4 ml[4];
         float2 x[4], y[4];
@@ -517,49 +544,97 @@ template <class E> __global__ __launch_bounds__(256) void attn_diff_join_kernel(
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             if (s0 + 4 * u >= shares) break;
-            const float m0 = fmaxf(m[0], ml[u].x), m1 = fmaxf(m[1], ml[u].z);
-            const float a0 = __builtin_amdgcn_exp2f(m[0] - m0), a1 = __builtin_amdgcn_exp2f(m[1] - m1), b0 = __builtin_amdgcn_exp2f(ml[u].x - m0), b1 = __builtin_amdgcn_exp2f(ml[u].z - m1);
-            m[0] = m0; m[1] = m1;
-            l[0] = fmaf(l[0], a0, ml[u].y * b0); l[1] = fmaf(l[1], a1, ml[u].w * b1);
-            o[0][0] = fmaf(o[0][0], a0, x[u].x * b0); o[0][1] = fmaf(o[0][1], a0, x[u].y * b0);
-            o[1][0] = fmaf(o[1][0], a1, y[u].x * b1); o[1][1] = fmaf(o[1][1], a1, y[u].y * b1);
+            sum.add(ml[u], x[u], y[u]);
         }
     }
-    if (lane == 0) { s_m[wave][0] = m[0]; s_m[wave][1] = m[1]; s_l[wave][0] = l[0]; s_l[wave][1] = l[1]; }
-    s_o[wave][0][lane] = o[0][0]; s_o[wave][1][lane] = o[0][1]; s_o[wave][2][lane] = o[1][0]; s_o[wave][3][lane] = o[1][1];
+    if (lane == 0) s_ml[wave] = make_float4(sum.m[0], sum.l[0], sum.m[1], sum.l[1]);
+    s_o[wave][0][lane] = make_float2(sum.o[0][0], sum.o[0][1]); s_o[wave][1][lane] = make_float2(sum.o[1][0], sum.o[1][1]);
     __syncthreads();
     if (wave) return;
+    Joined<E> all;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        m[i] = fmaxf(fmaxf(s_m[0][i], s_m[1][i]), fmaxf(s_m[2][i], s_m[3][i]));
-        l[i] = o[i][0] = o[i][1] = 0.f;
+    for (int w = 0; w < 4; ++w) all.add(s_ml[w], s_o[w][0][lane], s_o[w][1][lane]);
+    all.finish(p, b, h, row, lane, lam, g);
+}
+
+// A few rows and at most 256 keys: one workgroup per (sequence, key / value head), 32 keys to each of its eight waves, joined in LDS: one launch and no scratch memory.
+// 8 heads, 100 / 256 keys: 6.8 / 7.7 us in a graph, 11.3 called one by one; shares and join 9.7 / 9.1 and 15.5.  (More keys, as a loop over tiles: 513 keys 11.6 against 9.7 us.)
+constexpr int GROUP_WAVES = 8, GROUP_ROWS = 16, GROUP_KEYS = GROUP_WAVES * 32, GROUP_LDS = GROUP_WAVES * (64 * ROW_B + GROUP_ROWS * 16);
+template <class E> __global__ __launch_bounds__(GROUP_WAVES * 64, 2) void attn_diff_group_kernel(DiffArgs p) {
+    constexpr int TILE_B = 32 * ROW_B;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    float4* s_ml = (float4*)(smem + GROUP_WAVES * 2 * TILE_B);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = blockIdx.x % p.kv_heads, b = blockIdx.x / p.kv_heads, rows = p.n_q * p.group, row = lane & 31;
+    const int rc = min(row, rows - 1), q = rc / p.group, head = h * p.group + rc % p.group;
+    const int len = key_count(p, b), last = seen_by(p, b, len, p.n_q - 1), k0 = wave * 32;
+    const uint32_t sK = lds_addr_of(smem) + wave * 2 * TILE_B, sV = sK + TILE_B;
+    if (k0 < last) {          // requests as in the wave kernel; the keys, the values, the queries and lambda come in one wait
+        const svd_bf16* ks = p.K + b * p.k_sb + h * p.k_sh + k0 * p.k_st;
+        const svd_bf16* vs = p.V + b * p.v_sb + h * p.v_sh + k0 * p.v_st;
+        const int l4 = lane >> 4, c16 = lane & 15, top = min(31, last - 1 - k0);
+        const uint32_t k_row = (uint32_t)p.k_st * 2, v_row = (uint32_t)p.v_st * 2;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float a = __builtin_amdgcn_exp2f(s_m[w][i] - m[i]);
-            l[i] = fmaf(s_l[w][i], a, l[i]);
-            o[i][0] = fmaf(s_o[w][2 * i][lane], a, o[i][0]); o[i][1] = fmaf(s_o[w][2 * i + 1][lane], a, o[i][1]);
+        for (int r = 0; r < 32; r += 4) {
+            const uint32_t at = min(r + l4, top);
+            glds16_saddr(at * k_row + ((c16 ^ l4 ^ (r & 12)) << 4), ks, sK + r * ROW_B);
+            glds16_saddr(at * v_row + ((c16 ^ (l4 << 2)) << 4), vs, sV + r * ROW_B);
         }
     }
-    const float lam = diff_lambda(p.lam, p.lambda_init, lane);
-    const float w0 = l[0] == 0.f ? 0.f : 1.f / l[0], w1 = l[1] == 0.f ? 0.f : lam / l[1];
-    float y0 = o[0][0] * w0 - o[1][0] * w1, y1 = o[0][1] * w0 - o[1][1] * w1;
-    if (p.gamma) {
-        const float norm = diff_norm(wave_sum(fmaf(y0, y0, y1 * y1)), p);
-        y0 *= norm * p.gamma[2 * lane]; y1 *= norm * p.gamma[2 * lane + 1];
+    DiffWave<E> w;
+    w.init(p.Q + b * p.q_sb + q * p.q_st + head * p.q_sh, lane);
+    w.seen = seen_by(p, b, len, q);
+    w.first = seen_by(p, b, len, 0);
+    const float lam = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, diff_lambda(p.lam, p.lambda_init, lane))));          // one register less
+    w.clear();
+    if (k0 < last) {
+        svd_wait_dma();
+        w.template tile<false>(sK, sV, k0);
+        if (__builtin_amdgcn_ballot_w64(w.bad)) {
+            w.clear();
+            w.template tile<true>(sK, sV, k0);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    *(uint32_t*)(p.O + b * p.o_sb + (row / p.group) * p.o_st + (h * p.group + row % p.group) * p.o_sh + 2 * lane) = E::pack(y0, y1);
+    const float2 g = gamma_pair(p, lane);
+    w.join_halves();
+    // 16 rows of 1 KiB in the wave's own tiles, pieces of 16 bytes swizzled by the row
+    if (row < rows) {
+        float4* part = (float4*)(smem + wave * 2 * TILE_B) + row * 64;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                    part[((128 * i + 32 * t + 2 * r + 4 * w.hi) >> 2) ^ row] = make_float4(w.o[i][t][r], w.o[i][t][r + 1], w.o[i][t][r + 2], w.o[i][t][r + 3]);
+        if (w.hi == 0) s_ml[wave * GROUP_ROWS + row] = make_float4(w.m[0], w.l[0], w.m[1], w.l[1]);
+    }
+    __syncthreads();
+    for (int r = wave; r < rows; r += GROUP_WAVES) {
+        Joined<E> sum;
+#pragma unroll
+        for (int s = 0; s < GROUP_WAVES; ++s) {
+            const float* part = (const float*)(smem + s * 2 * TILE_B) + r * 256 + (lane & 1) * 2;
+            sum.add(s_ml[s * GROUP_ROWS + r], *(const float2*)(part + ((lane >> 1) ^ r) * 4), *(const float2*)(part + ((32 + (lane >> 1)) ^ r) * 4));
+        }
+        sum.finish(p, b, h, r, lane, lam, g);
+    }
 }
 
 // Which form: see svd_attn_diff
-struct Plan { bool waves; int row_blocks, shares; int64_t ws; };
+enum { ROWS, WAVES, GROUP };
+struct Plan { int form, row_blocks, shares; int64_t ws; };
 Plan plan_for(int64_t batch, int64_t n_q, int64_t n_k, int64_t heads, int64_t kv_heads) {
     const int64_t rows = n_q * (heads / kv_heads), bh = batch * kv_heads;
-    Plan r = {true, (int)((rows + 31) / 32), 1, 0};
-    if (rows > 64 && (rows + 127) / 128 * bh >= 128) return {false, (int)((rows + 127) / 128), 1, 0};
+    Plan r = {WAVES, (int)((rows + 31) / 32), 1, 0};
+    if (rows > 64 && (rows + 127) / 128 * bh >= 128) return {ROWS, (int)((rows + 127) / 128), 1, 0};
     const int64_t units = r.row_blocks * bh;
     if (units > 0) {
         int64_t shares = (1024 + units - 1) / units;          // four waves on each CU (8 caches of 16-32k keys: 100 us with 640 to 1280 waves, 105 with 2048, 130 with 4096)
         if (shares > (n_k + 63) / 64) shares = (n_k + 63) / 64;
+        // one launch where the keys fit one workgroup and there is a CU for each
+        if (shares > 1 && rows <= GROUP_ROWS && bh <= 256 && n_k <= GROUP_KEYS) return {GROUP, 1, 1, 0};
         if (shares > 1) { r.shares = (int)shares; r.ws = rows * bh * shares * PART * 4; }
     }
     return r;
@@ -594,11 +669,16 @@ extern "C" int svd_attn_diff(const svd_bf16* Q, int64_t q_sb, int64_t q_st, int6
                         n_q, n_k, kv_heads, group, causal};
     const int64_t grid = (int64_t)plan.row_blocks * batch * kv_heads * plan.shares;
     if (grid > 0x7fffffff || (int64_t)batch * heads * n_q > 0x7fffffff) return SVD_EINVAL;
-    if (!plan.waves) {
+    if (plan.form == ROWS) {
         constexpr int LDS = 8 * 32 * ROW_B + 4 * Q_B;          // rings and map 2's queries: 76 KiB, two workgroups on a CU (two of 80 do not fit)
         SVD_DISPATCH_DTYPE(dtype, {
             SVD_ALLOW_LDS(attn_diff_rows_kernel<E>, LDS);
             hipLaunchKernelGGL((attn_diff_rows_kernel<E>), dim3((unsigned)grid), dim3(256), LDS, (hipStream_t)stream, p, plan.row_blocks);
+        });
+    } else if (plan.form == GROUP) {
+        SVD_DISPATCH_DTYPE(dtype, {
+            SVD_ALLOW_LDS(attn_diff_group_kernel<E>, GROUP_LDS);
+            hipLaunchKernelGGL((attn_diff_group_kernel<E>), dim3((unsigned)grid), dim3(GROUP_WAVES * 64), GROUP_LDS, (hipStream_t)stream, p);
         });
     } else {
         const int LDS = (n_k > 32 ? 4 : 2) * 32 * ROW_B;          // one tile needs no second buffer: 8 waves on a CU instead of 5 (25 keys x 23040 heads: 182 us, 300 with two and rows written 8 bytes at a time)

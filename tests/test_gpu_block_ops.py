@@ -424,6 +424,28 @@ def test_attn_what_a_query_does_not_see_does_not_reach_it(ops, t, n):
             assert torch.isnan(got[:, at:]).any(-1).all()
 
 
+@pytest.mark.parametrize("t", [F16, BF16], ids=str)
+@pytest.mark.parametrize("causal", [False, True], ids=["all", "causal"])
+@pytest.mark.parametrize("B,n_q,n_k,H,KV", [(1, 1, 256, 8, 8), (2, 1, 255, 16, 1), (1, 16, 256, 2, 2), (3, 4, 129, 8, 2), (1, 1, 66, 1, 1), (5, 2, 200, 8, 1), (4, 1, 257, 4, 4), (3, 17, 250, 2, 2)])
+def test_attn_short_caches(ops, t, B, n_q, n_k, H, KV, causal):
+    """A few rows on up to 256 keys, lengths from none to all, whatever lies in what is not seen, and the largest scores in one wave's keys only."""
+    randn = gen(503)
+    q, k, v = randn(B, n_q, H, 128).to(t), randn(B, n_k, KV, 128).to(t), randn(B, n_k, KV, 128).to(t)
+    k[:, 40:44] *= 8
+    lens = [n_k, 0, 1, n_k // 2, 33][:B]
+    k2, v2 = k.clone(), v.clone()
+    for b, n in enumerate(lens):
+        k2[b, n:], v2[b, n:] = float("nan"), float("inf")
+    run_attn(ops, f"attn short caches {B} {n_q}x{n_k} {H}/{KV} {t}", q, k2, v2, 7, causal=causal, k_len=ints(*lens), k_ref=k, v_ref=v)
+    if causal:          # something not finite that only later queries see
+        lam = torch.zeros(4, 64, device="cuda")
+        want, bound = attn64(q, k, v, lam, 0.4, None, 1e-5, True, None, None)
+        v[:, n_k - 1] = float("nan")
+        got = ops.attn_diff(q, k, v, lam, 0.4, causal=True)
+        within("attn short caches: a NaN at the end", got[:, :-1], want[:, :-1], bound[:, :-1])
+        assert torch.isnan(got[:, -1]).all()
+
+
 @pytest.mark.parametrize("n_q", [1, 25, 150])
 def test_attn_views(ops, n_q):
     """Column ranges of a fused projection; (frame, pixel) rows; [batch, kv head, capacity, 128] caches; a strided destination whose surroundings stay."""
