@@ -54,7 +54,7 @@ __device__ __forceinline__ int seen_by(const DiffArgs& p, int b, int len, int q)
 }
 
 // What a query does not see must not reach it, and a weight of 0 is no help against an Inf or NaN in V: 0 * NaN is NaN.  In a tile that some of the block's
-// queries see further into than others, non-finite values are looked for; if there are any, the block starts over in a form that multiplies with V with zeros in
+// queries see further into than others (where all see the same keys, hidden places hold the last of them again), non-finite values are looked for; if there are any, the block starts over in a form that multiplies with V with zeros in
 // their places, and counts with a second product -- of the places with the 0 / 1 mask -- the non-finite values that each (channel, query) does see: those
 // results become NaN (what p * NaN, and inf - lambda inf, come to).  Starting over keeps the rare form's registers out of the loop that always runs.
 template <class E> struct NonFinite {
@@ -94,6 +94,7 @@ template <class E, bool Q_LDS = false> struct DiffWave {
     uint32_t pk[2][8], rest[4 * RESTS];        // weights in 16 bits; what map 1's lost
     float m[2], l[2];
     int l31, hi, seen, first;          // keys that this lane's query sees; the fewest that any query of the wave sees
+    bool uneven;                       // some query sees less than what is staged: places behind the staged keys repeat the last, which all others see
     bool bad;                          // a value that is not finite in a tile with hidden places
     uint32_t ka, va;                   // byte offsets of the lane's first K and V^T fragment in a 32-key tile; the others differ in bits 5..7 (K) and 6, 7 (V)
 
@@ -204,7 +205,7 @@ template <class E, bool Q_LDS = false> struct DiffWave {
             for (int e = 0; e < 8; ++e) weigh(i, e);
         }
         if constexpr (!CLEAR) {
-            if (partial) look_for_bad(sV);
+            if (partial && uneven) look_for_bad(sV);
 #pragma unroll
             for (int q = 0; q < 2; ++q)
 #pragma unroll
@@ -350,6 +351,7 @@ template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kern
     w.init(p.Q + b * p.q_sb + q * p.q_st + head * p.q_sh, lane, (uint4*)(smem + 2 * RING_B + wave * Q_B));
     w.seen = seen_by(p, b, len, q);
     w.first = seen_by(p, b, len, min(rows - 1, row0) / p.group);
+    w.uneven = w.first < last;
     const svd_bf16* Kb = p.K + b * p.k_sb + h * p.k_sh;
     const svd_bf16* Vb = p.V + b * p.v_sb + h * p.v_sh;
     // Requests: wave-uniform base in scalars, the lane's offset in 32 bits (32 rows of at most 2^26 bytes).  8 KiB by four waves: two instructions each.
@@ -401,7 +403,7 @@ template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kern
             if (j + 2 < steps) stage(vp, v_row, vo, j + 2, lds + RING_B);
             kp += 32 * p.k_st; vp += 32 * p.v_st;
             if (j < my_steps) {
-                if (__builtin_expect_with_probability(j * 32 + 32 > w.first, 0, 0.99)) w.look_for_bad(at_v(j));
+                if (__builtin_expect_with_probability(w.uneven && j * 32 + 32 > w.first, 0, 0.99)) w.look_for_bad(at_v(j));
                 w.half(0, j * 32, at_k(j), at_v(j > 0 ? j - 1 : 0));
                 w.half(1, j * 32, at_k(j + 1), at_v(j));
                 if (__builtin_expect_with_probability(j == my_steps - 1, 0, 0.99)) {
@@ -444,6 +446,7 @@ template <class E> __global__ __launch_bounds__(64, 2) void attn_diff_wave_kerne
     w.init(p.Q + b * p.q_sb + q * p.q_st + head * p.q_sh, lane);
     w.seen = seen_by(p, b, len, q);
     w.first = seen_by(p, b, len, rb * 32 / p.group);
+    w.uneven = w.first < last;
     const svd_bf16* Kb = p.K + b * p.k_sb + h * p.k_sh;
     const svd_bf16* Vb = p.V + b * p.v_sb + h * p.v_sh;
     // requests as in the rows kernel; one wave requests all 8 + 8 KiB
@@ -585,6 +588,7 @@ template <class E> __global__ __launch_bounds__(GROUP_WAVES * 64, 2) void attn_d
     w.init(p.Q + b * p.q_sb + q * p.q_st + head * p.q_sh, lane);
     w.seen = seen_by(p, b, len, q);
     w.first = seen_by(p, b, len, 0);
+    w.uneven = w.first < last;
     const float lam = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, diff_lambda(p.lam, p.lambda_init, lane))));          // one register less
     w.clear();
     if (k0 < last) {
