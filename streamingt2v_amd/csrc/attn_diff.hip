@@ -281,8 +281,7 @@ template <class E, bool Q_LDS = false> struct DiffWave {
     }
     // (A_1 - lambda A_2) V, the head's norm, one rounding.  A lane holds 64 channels of one row in pieces of four: the rows go through 8 KiB of the wave's LDS (slots
     // swizzled by the row) and leave as whole rows, four to an instruction.
-    __device__ __forceinline__ void finish(const DiffArgs& p, int b, int h, int row0, int rows, uint32_t buf, int lane) {
-        const float lam = diff_lambda(p.lam, p.lambda_init, lane);
+    __device__ __forceinline__ void finish(const DiffArgs& p, int b, int h, int row0, int rows, uint32_t buf, int lane, float lam) {
         join_halves();
         const float w0 = l[0] == 0.f ? 0.f : 1.f / l[0], w1 = l[1] == 0.f ? 0.f : lam / l[1];
         float ss = 0.f;
@@ -424,7 +423,7 @@ template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kern
             }
         }
     }
-    w.finish(p, b, h, row0, rows, lds + wave * SLOT_B, lane);
+    w.finish(p, b, h, row0, rows, lds + wave * SLOT_B, lane, diff_lambda(p.lam, p.lambda_init, lane));
 }
 
 // Few queries: one wave per (sequence, key / value head, 32 rows, share of the keys), no workgroup barrier; tiles of 32 keys, two in turn.  With one share
@@ -462,9 +461,12 @@ template <class E> __global__ __launch_bounds__(64, 2) void attn_diff_wave_kerne
             glds16_saddr(row * v_row + ((c16 ^ (l4 << 2)) << 4), vs, dst + TILE_B);
         }
     };
+    if (begin < end) stage(begin, 0);
+    // lambda while the first keys are on their way, not behind the last
+    const float lam = shares == 1 ? __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, diff_lambda(p.lam, p.lambda_init, lane)))) : 0.f;
     auto walk = [&]<bool CLEAR>() {
         w.clear();
-        if (begin < end) stage(begin, 0);
+        if (CLEAR && begin < end) stage(begin, 0);
         int cur = 0;
         for (int k0 = begin; k0 < end; k0 += KT, cur ^= 1) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // the reads of the tile that is overwritten next are done
@@ -484,7 +486,7 @@ template <class E> __global__ __launch_bounds__(64, 2) void attn_diff_wave_kerne
     }
     if (shares == 1) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        w.finish(p, b, h, rb * 32, rows, lds, lane);
+        w.finish(p, b, h, rb * 32, rows, lds, lane, lam);
         return;
     }
     w.join_halves();
