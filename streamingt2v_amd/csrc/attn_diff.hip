@@ -324,8 +324,8 @@ template <class E, bool Q_LDS = false> struct DiffWave {
 // matrix unit (24 instructions of 32 cycles), so the two have to run at once inside a wave.  The maps take turns: while map 1's weights of step j are made, the matrix unit
 // does map 2's scores of step j and its products with V of step j - 1; while map 2's weights are made, map 1's scores of step j + 1 and its products with V of step j.
 // So K is read a step ahead and V a step behind: rings of four 8-KiB slots each, requests two steps ahead, one barrier a step.
-// 2 x 9216 tokens, 5 heads, fp16: 797 us (0.82 PFLOP/s of the one-pass work, 0.95 with the rests' products; the clock falls to 1.9 GHz under it; 720 workgroups on 512
-// places leave the second round half empty).  Before the maps took turns: 828 us without the rests.  4 causal prompts of 1001 to 2001 tokens, 8 heads on 4: 82 us (104
+// 2 x 9216 tokens, 5 heads, fp16: 782 us (0.83 PFLOP/s of the one-pass work, 0.97 with the rests' products; the clock falls to 1.9 GHz under it; 720 workgroups on 512
+// places leave the second round half empty).  Before the maps took turns: 828 us without the rests.  4 causal prompts of 1001 to 2001 tokens, 8 heads on 4: 81 us (104
 // with long rows first everywhere).
 template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kernel(DiffArgs p, int row_blocks) {
     constexpr int SLOT_B = 32 * ROW_B, RING_B = 4 * SLOT_B;          // K ring, then V ring
@@ -427,7 +427,7 @@ template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kern
 }
 
 // Few queries: one wave per (sequence, key / value head, 32 rows, share of the keys), no workgroup barrier; tiles of 32 keys, two in turn.  With one share
-// the wave finishes the rows (2304 x 10 heads of 25 frames: 178 us, 3.3 TB/s; 16 KiB requested by each of 8 waves a CU); else it leaves maxima, sums and both accumulators in the scratch memory (fp32, [row][share][260]) for the join
+// the wave finishes the rows (2304 x 10 heads of 25 frames: 173 us, 3.4 TB/s; 16 KiB requested by each of 8 waves a CU); else it leaves maxima, sums and both accumulators in the scratch memory (fp32, [row][share][260]) for the join
 // (8 caches of 16 to 32 k keys, 16 heads on 4: 90 us, 4.7 TB/s, and 5 for the join; one of 1025 keys, 8 heads: 6 and 3).
 template <class E> __global__ __launch_bounds__(64, 2) void attn_diff_wave_kernel(DiffArgs p, int row_blocks, int shares, float* ws) {
     constexpr int KT = 32, TILE_B = KT * ROW_B, BUF_B = 2 * TILE_B;
@@ -687,7 +687,7 @@ extern "C" int svd_attn_diff(const svd_bf16* Q, int64_t q_sb, int64_t q_st, int6
             hipLaunchKernelGGL((attn_diff_group_kernel<E>), dim3((unsigned)grid), dim3(GROUP_WAVES * 64), GROUP_LDS, (hipStream_t)stream, p);
         });
     } else {
-        const int LDS = (n_k > 32 ? 4 : 2) * 32 * ROW_B;          // one tile needs no second buffer: 8 waves on a CU instead of 5 (25 keys x 23040 heads: 182 us, 300 with two and rows written 8 bytes at a time)
+        const int LDS = (n_k > 32 ? 4 : 2) * 32 * ROW_B;          // one tile needs no second buffer: 8 waves on a CU instead of 5 (25 keys x 23040 heads: 173 us, 300 with two and rows written 8 bytes at a time)
         SVD_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((attn_diff_wave_kernel<E>), dim3((unsigned)grid), dim3(64), LDS, (hipStream_t)stream, p, plan.row_blocks, plan.shares, (float*)ws));
         SVD_CHECK_LAUNCH("attn_diff");
         if (plan.shares > 1)

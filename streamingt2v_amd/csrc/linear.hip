@@ -114,8 +114,8 @@ template <int EB> __device__ __forceinline__ uint4 load_chunk(const char* row, i
 // W's rows lie in LDS as even, then odd columns of each 64: a lane's two tiles of such a block are two adjacent columns, so results leave (and residuals come) as
 // pairs, 32 lanes a contiguous 128 (fp32: 256) bytes of a row.
 // Measured, 256 x 256: bf16 28800 x 1280 x 5120 onto an fp32 stream 392 us (0.96 PFLOP/s; two whole rounds 320 us, the split third 43, the join 17), e4m3
-// 28800 x 5120 x 1280 with GELU 258 us (1.46 PFLOP/s).  The same loop without its requests and LDS reads takes 232 of the 320 us (1.47 PFLOP/s, what a large library
-// product reaches), without either of them 286; of the 258 us the epilogue is about 90: one workgroup fills a CU, so nothing runs beside it.
+// 28800 x 5120 x 1280 with GELU 264 us (1.43 PFLOP/s).  The same loop without its requests and LDS reads takes 232 of the 320 us (1.47 PFLOP/s, what a large library
+// product reaches), without either of them 286; of the 264 us the epilogue is about 90: one workgroup fills a CU, so nothing runs beside it.
 template <int WM_, int WN_, int TM_, int TN_> struct Tile {
     static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, WAVES = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32, SLOT = (BM + BN) * 128, REQ = (BM + BN) / 8 / WAVES;
 };
