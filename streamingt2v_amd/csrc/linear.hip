@@ -391,13 +391,16 @@ template <class Eo, class T> __global__ __launch_bounds__(T::WAVES * 64) void li
 // ---- few rows: 32 columns x 32 TM rows per workgroup, its eight waves take 64-byte steps of K in turn and add up through LDS.  No staging: the weights are read
 // once, straight into fragments, and what bounds it is latency and how many of their bytes are in flight; rows of any alignment.  One row of 1280 by 5120 columns, e4m3:
 // 5.0 us (6.6 MB, 1.3 TB/s); 77 x 1001 x 515 fp16: 11 us. ----
-template <class In, class Eo, int TM> __global__ __launch_bounds__(512) void linear_rows_kernel(LinArgs p, int tiles_n) {
-    constexpr int NW = 8;
+template <class In, class Eo, int TM, int NW> __global__ __launch_bounds__(NW * 64) void linear_rows_kernel(LinArgs p, int tiles_n, int cols) {
     __shared__ __attribute__((aligned(16))) float part[NW][TM * 16][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
-    const int m0 = (blockIdx.x / tiles_n) * 32 * TM, n0 = (blockIdx.x % tiles_n) * 32;
+    const int m0 = (blockIdx.x / tiles_n) * 32 * TM, n0 = (blockIdx.x % tiles_n) * cols;
+    const int wb = l31 < cols && n0 + l31 < p.N ? p.kbytes : 0;          // rows that do not count are zeros and cost no requests
     const char* wr = p.W + (int64_t)min(n0 + l31, p.N - 1) * p.ldw;
     const char* xr[TM];
+    int xb[TM];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) xb[i] = m0 + 32 * i + l31 < p.M ? p.kbytes : 0;
 #pragma unroll
     for (int i = 0; i < TM; ++i) xr[i] = p.X + (int64_t)min(m0 + 32 * i + l31, p.M - 1) * p.ldx;
     f32x16_t acc[TM];
@@ -414,9 +417,9 @@ template <class In, class Eo, int TM> __global__ __launch_bounds__(512) void lin
             const int kb = (j0 + u * NW) * 64 + 32 * hi;          // behind K: zeros
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                w[u][c] = load_chunk<In::kBytes>(wr, kb + 16 * c, p.kbytes);
+                w[u][c] = load_chunk<In::kBytes>(wr, kb + 16 * c, wb);
 #pragma unroll
-                for (int i = 0; i < TM; ++i) x[u][i][c] = load_chunk<In::kBytes>(xr[i], kb + 16 * c, p.kbytes);
+                for (int i = 0; i < TM; ++i) x[u][i][c] = load_chunk<In::kBytes>(xr[i], kb + 16 * c, xb[i]);
             }
         }
 #pragma unroll
@@ -437,7 +440,7 @@ template <class In, class Eo, int TM> __global__ __launch_bounds__(512) void lin
     __syncthreads();
     for (int o = tid; o < TM * 16 * 64; o += NW * 64) {
         const int r = o >> 6, ln = o & 63, m = m0 + 32 * (r >> 4) + 8 * ((r & 15) >> 2) + 4 * (ln >> 5) + (r & 3), n = n0 + (ln & 31);
-        if (m >= p.M || n >= p.N) continue;
+        if (m >= p.M || n >= p.N || (ln & 31) >= cols) continue;
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) v += part[w][r][ln];
@@ -448,6 +451,7 @@ template <class In, class Eo, int TM> __global__ __launch_bounds__(512) void lin
 using Big = Tile<2, 4, 4, 2>;              // 256 x 256, eight waves, 128 KiB: one workgroup on a CU
 using Small = Tile<2, 2, 2, 2>;            // 128 x 128, four waves, 64 KiB: two
 constexpr int CUS = 256;
+constexpr int ROWS_TWO = 256, COLS_MIN = 8;
 
 // Which form, from sizes alone.
 enum { ROWS, BIG, SMALL };
@@ -493,11 +497,17 @@ int64_t aligned_copy_bytes(int64_t M, int64_t N, int64_t kbytes) { return (M + N
 template <class In, class Eo> int launch(LinArgs p, void* ws, int64_t ws_bytes, hipStream_t stream) {
     const LinPlan plan = lin_plan(p.M, p.N, p.kbytes, In::kWiden);
     if (plan.form == ROWS) {
-        const int tm = p.M <= 32 ? 1 : 2;
-        const int64_t tn = (p.N + 31) / 32, grid = (p.M + 32 * tm - 1) / (32 * tm) * tn;
-        if (grid > 0x7fffffff) return SVD_EINVAL;
-        if (tm == 1) hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 1>), dim3((unsigned)grid), dim3(512), 0, stream, p, (int)tn);
-        else hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 2>), dim3((unsigned)grid), dim3(512), 0, stream, p, (int)tn);
+        int cols = 32;
+        const int64_t tm = (p.M + 31) / 32;
+        while (cols > COLS_MIN && (p.N + cols / 2 - 1) / (cols / 2) * tm <= CUS) cols /= 2;
+        const int64_t tn = (p.N + cols - 1) / cols, ones = tm * tn;
+        const bool two = p.M > 32 && ones > ROWS_TWO, many = p.kbytes > 2048 && ones <= ROWS_TWO;
+        const int64_t grid = two ? (p.M + 63) / 64 * tn : ones;
+        if (grid > 0x7fffff) return SVD_EINVAL;          // 2^32 threads
+        const dim3 g((unsigned)grid);
+        if (two) hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 2, 8>), g, dim3(512), 0, stream, p, (int)tn, cols);
+        else if (many) hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 1, 16>), g, dim3(1024), 0, stream, p, (int)tn, cols);
+        else hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 1, 8>), g, dim3(512), 0, stream, p, (int)tn, cols);
         SVD_CHECK_LAUNCH("linear_act");
         return SVD_OK;
     }
