@@ -388,33 +388,38 @@ template <class Eo, class T> __global__ __launch_bounds__(T::WAVES * 64) void li
     finish_tiles<Eo, 1, T::TN>(p, acc, m0, n0, s_xs[wave], m0 + 32 <= p.M, lane & 31, lane >> 5);
 }
 
-// ---- few rows: 32 columns x 32 TM rows per workgroup, its eight waves take 64-byte steps of K in turn and add up through LDS.  No staging: the weights are read
-// once, straight into fragments, and what bounds it is latency and how many of their bytes are in flight; rows of any alignment.  One row of 1280 by 5120 columns, e4m3:
-// 5.0 us (6.6 MB, 1.3 TB/s); 77 x 1001 x 515 fp16: 11 us. ----
-template <class In, class Eo, int TM, int NW> __global__ __launch_bounds__(NW * 64) void linear_rows_kernel(LinArgs p, int tiles_n, int cols) {
+// ---- few rows: 32 columns x 32 TM rows per workgroup, its waves take 64-byte steps of K in turn and add up through LDS.  No staging: the weights are read once, straight
+// into fragments; rows of any alignment.  What bounds it is latency and the rate at which a CU takes requests of 64 lanes, so the work is spread: 16 or 8 columns to a
+// workgroup while all of them are on the chip at once, sixteen waves for long rows.  A tile of 8 (16) columns and at most as many rows multiplies 4 (2) steps of K at once: the
+// 32 rows and columns of the matrix instruction are its rows and columns in `groups` different places of K, and only the products of the same place count.
+// us, before and after: 1 x 1280 x 5120 bf16 13.3 -> 6.0, e4m3 8.0 -> 4.5 (6.6 MB); 64 x 1280 x 5120 bf16 29 -> 17; 77 x 1001 x 515 fp16 11 -> 6.7; one row of 1280 by
+// 5120 columns, e4m3 4.2. ----
+template <class In, class Eo, int TM, int NW> __global__ __launch_bounds__(NW * 64) void linear_rows_kernel(LinArgs p, int tiles_n, int log_cols, int groups) {
+    const int cols = 1 << log_cols;
     __shared__ __attribute__((aligned(16))) float part[NW][TM * 16][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l31 = lane & 31, hi = lane >> 5;
-    const int m0 = (blockIdx.x / tiles_n) * 32 * TM, n0 = (blockIdx.x % tiles_n) * cols;
-    const int wb = l31 < cols && n0 + l31 < p.N ? p.kbytes : 0;          // rows that do not count are zeros and cost no requests
-    const char* wr = p.W + (int64_t)min(n0 + l31, p.N - 1) * p.ldw;
+    const int m0 = (blockIdx.x / tiles_n) * (groups > 1 ? cols : 32 * TM), n0 = (blockIdx.x % tiles_n) * cols;
+    const int kg = groups > 1 ? l31 >> log_cols : 0, lr = l31 - kg * cols;          // the lane's share of K and its row and column of the tile
+    const int wb = lr < cols && n0 + lr < p.N ? p.kbytes : 0;          // rows that do not count are zeros and cost no requests
+    const char* wr = p.W + (int64_t)min(n0 + lr, p.N - 1) * p.ldw;
     const char* xr[TM];
     int xb[TM];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) xb[i] = m0 + 32 * i + l31 < p.M ? p.kbytes : 0;
+    for (int i = 0; i < TM; ++i) xb[i] = m0 + 32 * i + lr < p.M ? p.kbytes : 0;
 #pragma unroll
-    for (int i = 0; i < TM; ++i) xr[i] = p.X + (int64_t)min(m0 + 32 * i + l31, p.M - 1) * p.ldx;
+    for (int i = 0; i < TM; ++i) xr[i] = p.X + (int64_t)min(m0 + 32 * i + lr, p.M - 1) * p.ldx;
     f32x16_t acc[TM];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][r] = 0.f;
     constexpr int U = TM == 1 ? 4 : 2;          // steps in flight
-    const int steps = (p.kbytes + 63) >> 6;
+    const int steps = (p.kbytes + 64 * groups - 1) / (64 * groups);
     for (int j0 = wave; j0 < steps; j0 += NW * U) {
         uint4 w[U][2], x[U][TM][2];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int kb = (j0 + u * NW) * 64 + 32 * hi;          // behind K: zeros
+            const int kb = ((j0 + u * NW) * groups + kg) * 64 + 32 * hi;          // behind K: zeros
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 w[u][c] = load_chunk<In::kBytes>(wr, kb + 16 * c, wb);
@@ -438,12 +443,16 @@ template <class In, class Eo, int TM, int NW> __global__ __launch_bounds__(NW * 
 #pragma unroll
         for (int r = 0; r < 16; ++r) part[wave][i * 16 + r][lane] = acc[i][r];
     __syncthreads();
-    for (int o = tid; o < TM * 16 * 64; o += NW * 64) {
-        const int r = o >> 6, ln = o & 63, m = m0 + 32 * (r >> 4) + 8 * ((r & 15) >> 2) + 4 * (ln >> 5) + (r & 3), n = n0 + (ln & 31);
-        if (m >= p.M || n >= p.N || (ln & 31) >= cols) continue;
+    const int log_w = groups > 1 ? log_cols : 5;
+    for (int o = tid; o < TM << 2 * log_w; o += NW * 64) {
+        const int c = o & ((1 << log_w) - 1), row = o >> log_w, m = m0 + row, n = n0 + c;
+        if (m >= p.M || n >= p.N || c >= cols) continue;
         float v = 0.f;
+        for (int g = 0; g < groups; ++g) {          // of the tile, the blocks whose row and column have the same share of K
+            const int x = row + g * cols, r = (x >> 3) * 4 + (x & 3), ln = ((x >> 2) & 1) * 32 + c + g * cols;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) v += part[w][r][ln];
+            for (int w = 0; w < NW; ++w) v += part[w][r][ln];
+        }
         epilogue<Eo>(p, m, n, v);
     }
 }
@@ -451,7 +460,7 @@ template <class In, class Eo, int TM, int NW> __global__ __launch_bounds__(NW * 
 using Big = Tile<2, 4, 4, 2>;              // 256 x 256, eight waves, 128 KiB: one workgroup on a CU
 using Small = Tile<2, 2, 2, 2>;            // 128 x 128, four waves, 64 KiB: two
 constexpr int CUS = 256;
-constexpr int ROWS_TWO = 256, COLS_MIN = 8;
+constexpr int ROWS_TWO = 256;
 
 // Which form, from sizes alone.
 enum { ROWS, BIG, SMALL };
@@ -497,17 +506,21 @@ int64_t aligned_copy_bytes(int64_t M, int64_t N, int64_t kbytes) { return (M + N
 template <class In, class Eo> int launch(LinArgs p, void* ws, int64_t ws_bytes, hipStream_t stream) {
     const LinPlan plan = lin_plan(p.M, p.N, p.kbytes, In::kWiden);
     if (plan.form == ROWS) {
-        int cols = 32;
+        // Columns to a workgroup: halved while every one still has a CU; two tiles of rows share the weights' fragments once there are more than that
+        // (64 x 1280 x 5120: 29 us with two, 17 without; 256 x 1280 x 5120: 33 and 42).
+        int log_cols = 5;
         const int64_t tm = (p.M + 31) / 32;
-        while (cols > COLS_MIN && (p.N + cols / 2 - 1) / (cols / 2) * tm <= CUS) cols /= 2;
+        while (log_cols > 3 && (((int64_t)p.N - 1 >> (log_cols - 1)) + 1) * tm <= CUS) --log_cols;
+        const int cols = 1 << log_cols;
+        const int groups = p.M <= cols && p.kbytes < 1 << 30 ? 32 / cols : 1;          // (positions in K stay 32-bit numbers)
         const int64_t tn = (p.N + cols - 1) / cols, ones = tm * tn;
-        const bool two = p.M > 32 && ones > ROWS_TWO, many = p.kbytes > 2048 && ones <= ROWS_TWO;
+        const bool two = p.M > 32 && ones > ROWS_TWO, many = p.kbytes > 2048 * groups && ones <= ROWS_TWO;
         const int64_t grid = two ? (p.M + 63) / 64 * tn : ones;
         if (grid > 0x7fffff) return SVD_EINVAL;          // 2^32 threads
         const dim3 g((unsigned)grid);
-        if (two) hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 2, 8>), g, dim3(512), 0, stream, p, (int)tn, cols);
-        else if (many) hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 1, 16>), g, dim3(1024), 0, stream, p, (int)tn, cols);
-        else hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 1, 8>), g, dim3(512), 0, stream, p, (int)tn, cols);
+        if (two) hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 2, 8>), g, dim3(512), 0, stream, p, (int)tn, log_cols, groups);
+        else if (many) hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 1, 16>), g, dim3(1024), 0, stream, p, (int)tn, log_cols, groups);
+        else hipLaunchKernelGGL((linear_rows_kernel<In, Eo, 1, 8>), g, dim3(512), 0, stream, p, (int)tn, log_cols, groups);
         SVD_CHECK_LAUNCH("linear_act");
         return SVD_OK;
     }

@@ -240,6 +240,28 @@ def test_linear_sizes(ops, t):
         check_linear(f"linear {m}x{n}x{k} {t} {act}", got, x, w, sx, sw, bias, act, res)
 
 
+FEW_ROWS = [(1, 1280, 5120), (8, 1280, 2560), (9, 1280, 2560), (16, 2560, 320), (17, 2560, 320), (3, 9, 5117), (8, 2048, 64), (5, 321, 63), (1, 2049, 65), (16, 4096, 1029), (64, 512, 4096), (33, 100, 129)]
+
+
+@pytest.mark.parametrize("t", [F16, BF16, F8], ids=str)
+def test_linear_few_rows(ops, t):
+    """Every number of columns to a workgroup, and K shorter and longer than what its waves take at once; a NaN in one row or column stays there."""
+    for i, (m, n, k) in enumerate(FEW_ROWS):
+        randn, x, w, sx, sw = make_linear(260 + i, m, n, k, t)
+        e = BF16 if t == F8 else t
+        for od in (e, F32):
+            got = ops.linear_act(x, w, act="silu", x_scale=sx, w_scale=sw, out_dtype=od)
+            check_linear(f"linear {m}x{n}x{k} {t} {od}", got, x, w, sx, sw, None, "silu", None)
+        x2, w2 = x.clone(), w.clone()
+        x2.view(torch.uint8)[m // 2].fill_(0x7f)          # NaN in e4m3 and bf16, fp16 (0x7f7f)
+        w2.view(torch.uint8)[n // 3].fill_(0x7f)
+        bad = ops.linear_act(x2, w2, act="silu", x_scale=sx, w_scale=sw, out_dtype=e)
+        same = ops.linear_act(x, w, act="silu", x_scale=sx, w_scale=sw, out_dtype=e)
+        keep = torch.ones(m, n, dtype=torch.bool, device="cuda")
+        keep[m // 2], keep[:, n // 3] = False, False
+        assert torch.equal(bad[keep], same[keep])
+
+
 @pytest.mark.parametrize("act", list(ACTS))
 @pytest.mark.parametrize("t", [F16, F8], ids=str)
 def test_linear_activations_reach_far_values(ops, act, t):
