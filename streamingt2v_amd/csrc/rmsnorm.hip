@@ -14,6 +14,11 @@ __device__ __forceinline__ float f8_scale(float row_max, float square_sum) {
     return !(square_sum < INFINITY) ? NAN : row_max == 0.f ? 0.f : fmaxf(row_max / F8_MAX, 0x1p-126f);
 }
 __device__ __forceinline__ float f8_inv(float a) { return a == 0.f ? 0.f : 1.f / a; }
+// 1 / sqrt(mean(s^2) + eps); a row of zeros stays zeros with eps = 0 too
+__device__ __forceinline__ float rms_inv(float square_sum, int channels, float eps) {
+    const float d = square_sum / (float)channels + eps;
+    return d == 0.f ? 0.f : 1.f / sqrtf(d);
+}
 
 // Rows wider than 10240 channels, and fp32 x with a 16-bit residual.  One workgroup per row, any width: three passes over the row (square sum, maximum, result); the second and third read from the L2.
 // r and s may be the same rows: a thread reads the elements it writes, in every pass, and writes them last.
@@ -34,7 +39,7 @@ __global__ __launch_bounds__(256) void rmsnorm_row_kernel(const void* X, int64_t
         if ((tid & 63) == 0) red[wave] = sq;
         __syncthreads();
         const float ss = red[0] + red[1] + red[2] + red[3];
-        const float rstd = 1.f / sqrtf(ss / (float)channels + eps);
+        const float rstd = rms_inv(ss, channels, eps);
         float inv = 1.f;
         if constexpr (F8) {
             float mx = 0.f;
@@ -174,7 +179,7 @@ __global__ __launch_bounds__(256) void rmsnorm_vec_kernel(const void* X, int64_t
             }
         }
     const float ss = row_reduce<TPR, false>(sq, red);
-    const float rstd = 1.f / sqrtf(ss / (float)channels + eps);
+    const float rstd = rms_inv(ss, channels, eps);
     float mx = 0.f;
 #pragma unroll
     for (int k = 0; k < MAXV; ++k) {
