@@ -388,7 +388,7 @@ int svd_vfi_tta_average(const float* pred2, float* out, uint8_t* out_u8, int32_t
  *   X [rows][ldx]  16-bit `dtype`, or fp32 with SVD_RMS_X_F32.     R [rows][ldr] or NULL: 16-bit, or fp32 with SVD_RMS_R_F32.
  *   S [rows][lds] or NULL: the sum s, in R's type (needs R; S == R with lds == ldr updates the residual stream in place).
  *   Y [rows][ldy]  16-bit `dtype`; with SVD_RMS_OUT_F8 e4m3 values and yscale[rows] fp32: y = yscale[row] * Y[row], yscale = max |y| / 448, at least
- *     2^-126 (0 for a row of zeros; NaN, with NaN values, for a row whose square sum is not finite in fp32).
+ *     2^-126 (0 for a row of zeros; NaN, with NaN values, for a row with an Inf or NaN in it or in its sum).
  *   gamma [channels] fp32 or NULL (1).  Any channels from 1 to 2^31 - 256, any alignment and leading dimension of whole elements.  rows == 0 returns SVD_OK. */
 enum { SVD_RMS_X_F32 = 1, SVD_RMS_R_F32 = 2, SVD_RMS_OUT_F8 = 4 };
 int svd_rmsnorm(const void* X, int64_t ldx, const void* R, int64_t ldr, const float* gamma, float eps, void* Y, int64_t ldy, float* yscale,

@@ -7,18 +7,13 @@ namespace {
 
 constexpr float F8_MAX = 448.f;              // largest finite e4m3
 
-// The row's scale.  A row of zeros has scale 0 and values 0; a row whose square sum is not finite (an Inf or NaN in it, or |s| beyond 1e19) has scale NaN
+// The row's scale.  A row of zeros has scale 0 and values 0; a row with an Inf or NaN in it (or whose sum s overflows) has scale NaN
 // and values NaN, so that it cannot pass for numbers.  |y * inv| <= 448 (1 + 2^-22) rounds to at most 448: no clamp (which would swallow a NaN).
 // The scale of any other row is at least 2^-126: 1 / a of a smaller one would be infinite.
 __device__ __forceinline__ float f8_scale(float row_max, float square_sum) {
     return !(square_sum < INFINITY) ? NAN : row_max == 0.f ? 0.f : fmaxf(row_max / F8_MAX, 0x1p-126f);
 }
 __device__ __forceinline__ float f8_inv(float a) { return a == 0.f ? 0.f : 1.f / a; }
-// 1 / sqrt(mean(s^2) + eps); a row of zeros stays zeros with eps = 0 too
-__device__ __forceinline__ float rms_inv(float square_sum, int channels, float eps) {
-    const float d = square_sum / (float)channels + eps;
-    return d == 0.f ? 0.f : 1.f / sqrtf(d);
-}
 
 // Rows wider than 10240 channels, and fp32 x with a 16-bit residual.  One workgroup per row, any width: three passes over the row (square sum, maximum, result); the second and third read from the L2.
 // r and s may be the same rows: a thread reads the elements it writes, in every pass, and writes them last.
@@ -38,12 +33,22 @@ __global__ __launch_bounds__(256) void rmsnorm_row_kernel(const void* X, int64_t
         sq = wave_sum(sq);
         if ((tid & 63) == 0) red[wave] = sq;
         __syncthreads();
-        const float ss = red[0] + red[1] + red[2] + red[3];
-        const float rstd = rms_inv(ss, channels, eps);
+        float ss = red[0] + red[1] + red[2] + red[3];
+        const float f = svd_rms_factor(ss, eps);
+        if (f != 1.f) {
+            __syncthreads();
+            sq = 0.f;
+            for (int c = tid; c < channels; c += 256) { const float v = at(row, c) * f; sq = fmaf(v, v, sq); }
+            sq = wave_sum(sq);
+            if ((tid & 63) == 0) red[wave] = sq;
+            __syncthreads();
+            ss = red[0] + red[1] + red[2] + red[3];
+        }
+        const float rstd = svd_rms_inv(ss, (float)channels, eps * f * f);
         float inv = 1.f;
         if constexpr (F8) {
             float mx = 0.f;
-            for (int c = tid; c < channels; c += 256) mx = fmaxf(mx, fabsf(at(row, c) * (gamma ? gamma[c] * rstd : rstd)));
+            for (int c = tid; c < channels; c += 256) mx = fmaxf(mx, fabsf(at(row, c) * f * (gamma ? gamma[c] * rstd : rstd)));
             mx = wave_max(mx);
             if ((tid & 63) == 0) red[4 + wave] = mx;
             __syncthreads();
@@ -54,7 +59,7 @@ __global__ __launch_bounds__(256) void rmsnorm_row_kernel(const void* X, int64_t
         }
         for (int c = tid; c < channels; c += 256) {
             const float v = at(row, c);
-            const float y = v * (gamma ? gamma[c] * rstd : rstd);
+            const float y = v * f * (gamma ? gamma[c] * rstd : rstd);
             if constexpr (F8) {
                 const float q = y * inv;
                 ((uint8_t*)Y)[row * ldy + c] = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(q, q, 0, false);
@@ -178,8 +183,20 @@ __global__ __launch_bounds__(256) void rmsnorm_vec_kernel(const void* X, int64_t
                 if (c < channels) store8<E, RM == 2, AL>((char*)S + row * lds * (RM == 2 ? 4 : 2), c, channels, v[k]);
             }
         }
-    const float ss = row_reduce<TPR, false>(sq, red);
-    const float rstd = rms_inv(ss, channels, eps);
+    float ss = row_reduce<TPR, false>(sq, red);
+    const float f = svd_rms_factor(ss, eps);
+    if (__builtin_expect(f != 1.f, 0)) {          // all threads of the row
+        if (TPR > 64) __syncthreads();
+        sq = 0.f;
+#pragma unroll
+        for (int k = 0; k < MAXV; ++k)
+            if ((sub + TPR * k) * 8 < channels) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { v[k][i] *= f; sq = fmaf(v[k][i], v[k][i], sq); }
+            }
+        ss = row_reduce<TPR, false>(sq, red);
+    }
+    const float rstd = svd_rms_inv(ss, (float)channels, eps * f * f);
     float mx = 0.f;
 #pragma unroll
     for (int k = 0; k < MAXV; ++k) {

@@ -61,6 +61,18 @@ __device__ __forceinline__ svd_f32x2 gelu_erf_f2(svd_f32x2 x) {
     return __builtin_elementwise_fma(-ax, q, mx);
 }
 
+// RMS statistics of values whose squares leave fp32 (|v| beyond 1e19, or below 1e-20 with an eps that does not cover it): the power of two that brings them back, 1 for all
+// others.  The caller multiplies its values by it, sums the squares anew and takes eps f^2; v / sqrt(mean(v^2) + eps) does not change.  A square sum below 2^-80 has
+// values below 2^-40, 2^60 after the factor 2^100; one that overflowed has a value beyond 2^48 (2^31 of them), at least 2^-52 after 2^-100.  Inf and NaN stay what they are.
+__device__ __forceinline__ float svd_rms_factor(float square_sum, float eps) {
+    return !(square_sum < INFINITY) ? 0x1p-100f : square_sum < 0x1p-80f && eps < 0x1p-80f ? 0x1p100f : 1.f;
+}
+// 1 / sqrt(mean(v^2) + eps); 0 for values of zero with eps = 0: zeros stay zeros
+__device__ __forceinline__ float svd_rms_inv(float square_sum, float n, float eps) {
+    const float d = square_sum / n + eps;
+    return d == 0.f ? 0.f : 1.f / sqrtf(d);
+}
+
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
