@@ -340,8 +340,8 @@ __global__ __launch_bounds__(256, 1) void ff_geglu_fused_kernel(const svd_bf16* 
                 {   // GELU pair p = i / 5 (tile p / 4, registers 2 (p % 4), + 1), stage i % 5: the arithmetic of gelu_erf_f2 (svd_common.h), bit for bit
                     const int pr = i / 5, st = i % 5, t = pr >> 2, e = 2 * (pr & 3);
                     if (st == 0) {
-                        asm("v_min_f32 %0, %2, |%1|" : "=v"(gt[0]) : "v"(sc[t][8 + e]), "s"(7.0f));
-                        asm("v_min_f32 %0, %2, |%1|" : "=v"(gt[1]) : "v"(sc[t][9 + e]), "s"(7.0f));
+                        asm("v_minimum3_f32 %0, |%1|, %2, %2" : "=v"(gt[0]) : "v"(sc[t][8 + e]), "s"(7.0f));
+                        asm("v_minimum3_f32 %0, |%1|, %2, %2" : "=v"(gt[1]) : "v"(sc[t][9 + e]), "s"(7.0f));
                         asm("v_max_f32 %0, 0, %1" : "=v"(gmx[0]) : "v"(sc[t][8 + e]));
                         asm("v_max_f32 %0, 0, %1" : "=v"(gmx[1]) : "v"(sc[t][9 + e]));
                         gr = __builtin_elementwise_fma(k6, gt, k5);
@@ -355,9 +355,7 @@ __global__ __launch_bounds__(256, 1) void ff_geglu_fused_kernel(const svd_bf16* 
                         const svd_f32x2 ex = __builtin_elementwise_fma(gr, gt, km1);
                         gq[0] = __builtin_amdgcn_exp2f(ex[0]); gq[1] = __builtin_amdgcn_exp2f(ex[1]);
                     } else {
-                        svd_f32x2 ax;
-                        ax[0] = __builtin_fabsf(sc[t][8 + e]); ax[1] = __builtin_fabsf(sc[t][9 + e]);
-                        const svd_f32x2 gl = __builtin_elementwise_fma(-ax, gq, gmx);
+                        const svd_f32x2 gl = __builtin_elementwise_fma(-gt, gq, gmx);
                         hp[pr] = E::pack(sc[t][e] * gl[0], sc[t][e + 1] * gl[1]);
                     }
                 }
@@ -573,8 +571,8 @@ __global__ __launch_bounds__(512, 1) void ff_geglu_fused8_kernel(const svd_bf16*
                 {   // GELU pair pr = i / 5 (registers 2 pr, 2 pr + 1: value; 8 + 2 pr, 9 + 2 pr: gate), stage i % 5: gelu_erf_f2 (svd_common.h), bit for bit
                     const int pr = i / 5, st = i % 5, e = 2 * pr;
                     if (st == 0) {
-                        asm("v_min_f32 %0, %2, |%1|" : "=v"(gt[0]) : "v"(sc[8 + e]), "s"(7.0f));
-                        asm("v_min_f32 %0, %2, |%1|" : "=v"(gt[1]) : "v"(sc[9 + e]), "s"(7.0f));
+                        asm("v_minimum3_f32 %0, |%1|, %2, %2" : "=v"(gt[0]) : "v"(sc[8 + e]), "s"(7.0f));
+                        asm("v_minimum3_f32 %0, |%1|, %2, %2" : "=v"(gt[1]) : "v"(sc[9 + e]), "s"(7.0f));
                         asm("v_max_f32 %0, 0, %1" : "=v"(gmx[0]) : "v"(sc[8 + e]));
                         asm("v_max_f32 %0, 0, %1" : "=v"(gmx[1]) : "v"(sc[9 + e]));
                         gr = __builtin_elementwise_fma(k6, gt, k5);
@@ -588,9 +586,7 @@ __global__ __launch_bounds__(512, 1) void ff_geglu_fused8_kernel(const svd_bf16*
                         const svd_f32x2 ex = __builtin_elementwise_fma(gr, gt, km1);
                         gq[0] = __builtin_amdgcn_exp2f(ex[0]); gq[1] = __builtin_amdgcn_exp2f(ex[1]);
                     } else {
-                        svd_f32x2 ax;
-                        ax[0] = __builtin_fabsf(sc[8 + e]); ax[1] = __builtin_fabsf(sc[9 + e]);
-                        const svd_f32x2 gl = __builtin_elementwise_fma(-ax, gq, gmx);
+                        const svd_f32x2 gl = __builtin_elementwise_fma(-gt, gq, gmx);
                         hp[pr] = E::pack(sc[e] * gl[0], sc[e + 1] * gl[1]);
                     }
                 }

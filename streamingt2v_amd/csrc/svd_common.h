@@ -16,11 +16,12 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 // x * sigmoid(x) with the hardware reciprocal (1 ulp) instead of an IEEE division (v_div_scale / v_div_fmas / v_div_fixup: ~10 VALU):
 // every consumer rounds the result to 16 bit or feeds a sampler step; the GroupNorm+SiLU pass is no longer VALU-co-bound.
 __device__ __forceinline__ float silu_f(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
-// exact-erf GELU of the reference's GEGLU (attention.py:99-101):  gelu(x) = x Phi(x) = max(x, 0) - |x| q(|x|),  q(t) = Phi(-t) = 2^(r(t) - 1),
-// r(t) = log2 erfc(t / sqrt 2) by a degree-6 polynomial without constant term (weighted minimax fit on [0, 7], |erf error| <= 2.3e-7; q(7) is
-// 6e-13, so t is clamped there).  ONE transcendental (v_exp_f32) per element against two (rcp + exp2) for the Abramowitz-Stegun 7.1.26 form used before, no sign
-// transfer, and the relative accuracy of the negative tail comes for free: |gelu error| <= 2e-6 absolute over the whole fp32 range (numpy
-// float32 emulation of this exact sequence), i.e. 1/100 of the 16-bit output rounding.  The GEGLU epilogue of the ff1 GEMMs is bound by
+// exact-erf GELU of the reference's GEGLU (attention.py:99-101):  gelu(x) = x Phi(x) = max(x, 0) - t q(t),  t = |x|,  q(t) = Phi(-t) = 2^(r(t) - 1),
+// r(t) = log2 erfc(t / sqrt 2) by a degree-6 polynomial without constant term (weighted minimax fit on [0, 7], |erf error| <= 2.3e-7).  Behind 7, t stays 7 in the polynomial
+// AND in the product: 7 q(7) = 6.5e-12 is what is left of a function that has 9e-12 there and 0 in the limit (an unclamped |x| q(7) would grow with |x|).
+// ONE transcendental (v_exp_f32) per element against two (rcp + exp2) for the Abramowitz-Stegun 7.1.26 form used before, no sign
+// transfer, and the relative accuracy of the negative tail comes for free: |gelu error| <= 2e-6 absolute over the whole fp32 range, besides the rounding of a
+// large result (numpy float32 emulation of this exact sequence), i.e. 1/100 of the 16-bit output rounding; +inf gives +inf, -inf the limit 0, NaN NaN.  The GEGLU epilogue of the ff1 GEMMs is bound by
 // exactly this arithmetic (VALU is per SIMD: both waves' 64 gate values per lane serialise; round-2 ISA audit).
 __device__ __forceinline__ float gelu_erf_f(float x) {
     const float t = fminf(fabsf(x), 7.0f);
@@ -30,7 +31,7 @@ __device__ __forceinline__ float gelu_erf_f(float x) {
     r = fmaf(r, t, -4.590827371e-01f);
     r = fmaf(r, t, -1.151116856e+00f);
     const float q = __builtin_amdgcn_exp2f(fmaf(r, t, -1.0f));
-    return fmaf(-fabsf(x), q, fmaxf(x, 0.0f));
+    return fmaf(-t, q, x < 0.0f ? 0.0f : x);          // (a comparison keeps the NaN that fminf drops)
 }
 
 // The same function on a PAIR (round 4; the GEGLU epilogue of the ff1 GEMMs evaluates 64 of them per lane and output tile and is bound by this VALU
@@ -41,12 +42,11 @@ __device__ __forceinline__ float gelu_erf_f(float x) {
 // Round-3 ISA: ~17 instructions per element; this form saves the five plain ones.
 typedef float svd_f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ svd_f32x2 gelu_erf_f2(svd_f32x2 x) {
-    svd_f32x2 t, mx, ax;
-    asm("v_min_f32 %0, %2, |%1|" : "=v"(t[0]) : "v"(x[0]), "s"(7.0f));   // min(|x|, 7); the VOP3 form (|.| modifier) takes no literal: 7.0 in an SGPR
-    asm("v_min_f32 %0, %2, |%1|" : "=v"(t[1]) : "v"(x[1]), "s"(7.0f));
+    svd_f32x2 t, mx;
+    asm("v_minimum3_f32 %0, |%1|, %2, %2" : "=v"(t[0]) : "v"(x[0]), "s"(7.0f));   // min(|x|, 7), NaN for NaN (v_min_f32 gives 7); VOP3 takes no literal: 7.0 in an SGPR
+    asm("v_minimum3_f32 %0, |%1|, %2, %2" : "=v"(t[1]) : "v"(x[1]), "s"(7.0f));
     asm("v_max_f32 %0, 0, %1" : "=v"(mx[0]) : "v"(x[0]));                 // max(x, 0)
     asm("v_max_f32 %0, 0, %1" : "=v"(mx[1]) : "v"(x[1]));
-    ax[0] = __builtin_fabsf(x[0]); ax[1] = __builtin_fabsf(x[1]);
     const svd_f32x2 c6 = {1.775515804e-05f, 1.775515804e-05f}, c5 = {-6.477575890e-04f, -6.477575890e-04f}, c4 = {7.724042874e-03f, 7.724042874e-03f},
                     c3 = {-5.292673725e-02f, -5.292673725e-02f}, c2 = {-4.590827371e-01f, -4.590827371e-01f}, c1 = {-1.151116856e+00f, -1.151116856e+00f},
                     m1 = {-1.0f, -1.0f};
@@ -58,7 +58,7 @@ __device__ __forceinline__ svd_f32x2 gelu_erf_f2(svd_f32x2 x) {
     const svd_f32x2 e = __builtin_elementwise_fma(r, t, m1);
     svd_f32x2 q;
     q[0] = __builtin_amdgcn_exp2f(e[0]); q[1] = __builtin_amdgcn_exp2f(e[1]);
-    return __builtin_elementwise_fma(-ax, q, mx);
+    return __builtin_elementwise_fma(-t, q, mx);
 }
 
 // RMS statistics of values whose squares leave fp32 (|v| beyond 1e19, or below 1e-20 with an eps that does not cover it): the power of two that brings them back, 1 for all

@@ -1,10 +1,12 @@
 """RMS norm, linear with activation and differential attention at the ends of the numbers' range (-m gpu), against plain implementations in 64 bits.
 
 Bounds: those of test_gpu_block_ops (U32 = 2^-24 is one fp32 rounding, u(t) one rounding to t, tiny(t) half the type's smallest number) unless a test derives its own."""
+import math
+
 import pytest
 import torch
 
-from tests.test_gpu_block_ops import BF16, F16, F32, check_norm, gen, ops  # noqa: F401
+from tests.test_gpu_block_ops import BF16, F16, F32, F8, U32, check_norm, gen, ops, tiny, u, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +46,39 @@ def test_rmsnorm_rows_whose_squares_leave_fp32(ops, eps, f8):
             r = (randn(9, ch).clamp(-8, 8) * size).to(rt) if rt is not None else None
             gamma = 1 + randn(ch, scale=0.1) if i % 2 else None
             check_norm(f"rmsnorm squares out of range {ch} {xt} {rt}", ops.rmsnorm(x, gamma, eps=eps, residual=r, f8=f8), x, r, gamma, eps, f8)
+
+
+# ---------------------------------------------------------------------------------------------------------- linear_act
+FAR = [0.0, -0.0, 1e-30, -1e-30, 1.0, -1.0, 6.99, -6.99, 7.0, -7.0, 7.01, -7.01, 50.0, -50.0, 1e4, -1e4, 1e7, -1e7, 1e9, -1e9, 1e12, -1e12, 1e30, -1e30, 3e38, -3e38]
+
+
+@pytest.mark.parametrize("t", [F16, BF16, F8], ids=str)
+@pytest.mark.parametrize("m,n,k", [(1, 300, 64), (40, 300, 700), (300, 1040, 128), (300, 1041, 128), (1100, 1040, 2064), (1101, 1041, 2067), (4400, 2100, 64)])
+def test_linear_gelu_far_out(ops, t, m, n, k):
+    """x = 0, so the bias alone is the activation's argument, to both ends of fp32 and beyond.  gelu is within 2e-6 of x Phi(x) over the whole range, and one rounding; +inf gives
+    +inf, -inf the limit 0, NaN NaN."""
+    x, w = torch.zeros(m, k, device="cuda").to(t), gen(940)(n, k).to(t)
+    bias = torch.tensor(FAR, device="cuda").repeat(-(-n // len(FAR)))[:n].contiguous()
+    bias[n - 1], bias[n // 2], bias[n // 3] = float("inf"), float("-inf"), float("nan")
+    want = 0.5 * bias.double() * torch.erfc(-bias.double() / math.sqrt(2.0))
+    want[n // 2] = 0.0
+    for od in (F32, BF16 if t == F8 else t):
+        got = ops.linear_act(x, w, bias=bias, act="gelu", out_dtype=od)
+        same = torch.nan_to_num(got.float(), nan=0.125, posinf=0.375, neginf=-0.375)
+        assert torch.equal(same, same[:1].expand(m, n)), "every row is the same"
+        fits = want.abs() < torch.finfo(od).max          # (an fp16 result overflows to infinity behind 65504)
+        fits[n - 1] = fits[n // 3] = True
+        bound = 2e-6 + (u(od) + U32) * torch.nan_to_num(want.abs(), posinf=0.0) + tiny(od)
+        within(f"gelu far out {m}x{n}x{k} {t} {od}", got[0][fits], want[fits], bound[fits])
+
+
+def test_gelu_rows_far_out(ops):
+    """The row pass on every finite 16-bit number and the infinities: within 2e-6 and one rounding of x Phi(x)."""
+    for t in (F16, BF16):
+        x = torch.arange(65536, device="cuda").to(torch.int32).to(torch.int16).view(t).reshape(256, 256)
+        nan, inf = torch.isnan(x), torch.isinf(x)
+        xd = x.double()
+        want = torch.where(inf, xd.clamp_min(0), 0.5 * xd * torch.erfc(-xd / math.sqrt(2.0)))
+        got = ops.gelu_(x.clone())
+        bound = 2e-6 + (u(t) + U32) * torch.nan_to_num(want.abs(), nan=0.0, posinf=0.0) + tiny(t)
+        within(f"gelu rows {t}", got, torch.where(nan, xd, want), bound)
