@@ -8,7 +8,7 @@
 //                                      between the halves of the wave;
 //   O_i^T[channel][query] += V^T P_i^T  the accumulator registers 8 s .. 8 s + 7 of S_i^T are the B operand of step s as they stand, if the A operand holds
 //                                      the same keys in the same order: half h holds keys 16 s + 4 h + (0..3) and 16 s + 8 + 4 h + (0..3).
-// P is rounded to the 16-bit type for the matrix cores (at most half a step of the type relative to each weight); scores, maxima, sums and both accumulators
+// P is rounded to the 16-bit type for the matrix cores (at most half a step of the type relative to each weight, in fp16 at least 2^-32 of the row's largest); scores, maxima, sums and both accumulators
 // are fp32, and the row sums add the unrounded weights.  The maps' difference makes these roundings weigh more than the result's own (lambda 0.8, scores of
 // deviation 1: together 1.6 roundings of the result in the 2-norm), so what map 1's weights lose is rounded once more and multiplied as well: for all keys where the keys
 // and values are what takes the time (1.1 to 1.2 roundings), for 16 of 32 where the products are (1.45 at most; none, half, all of them: 727, 804, 896 us for 2 x 9216 tokens when it was measured).
@@ -88,11 +88,12 @@ __device__ __forceinline__ float halves_max(float v) {
 // Q_LDS: three of map 2's four query fragments wait in the wave's 3 KiB of LDS instead of 12 registers
 template <class E, bool Q_LDS = false> struct DiffWave {
     static constexpr int RESTS = Q_LDS ? 1 : 2;          // 16-key halves of a step whose weights' rests are multiplied
+    static constexpr float LIFT = E::kId == SVD_DTYPE_F16 ? 7.f : 0.f;          // see follow
     uint4 qf[8];
     uint4* q_lds;
     f32x16_t o[2][4], s[2];
     uint32_t pk[2][8], rest[4 * RESTS];        // weights in 16 bits; what map 1's lost
-    float m[2], l[2];
+    float m[2], l[2];                  // exponent that the weights are taken against, and their sum
     int l31, hi, seen, first;          // keys that this lane's query sees; the fewest that any query of the wave sees
     bool uneven;                       // some query sees less than what is staged: places behind the staged keys repeat the last, which all others see
     bool bad;                          // a value that is not finite in a tile with hidden places
@@ -155,11 +156,14 @@ template <class E, bool Q_LDS = false> struct DiffWave {
         for (int r = 2; r < 16; ++r) mx = fmaxf(mx, s[i][r]);
         return halves_max(mx) * C_EXP;
     }
-    // The maximum is only there to keep the weights in range: it follows when some query of the wave is 2^8 behind (weights up to 2^8 are as exact as weights up
-    // to 1), not at every new maximum, of which 64 rows have one in almost every tile of the first 2000 keys.  64 multiplications each time.
+    // m is the exponent that the weights are taken against.  It is only there to keep them in range: it follows when some query of the wave has a score 2^8 beyond
+    // what m last came from (weights that much larger are as exact as others), not at every new maximum, of which 64 rows have one in almost every tile of the first
+    // 2000 keys.  64 multiplications each time.  fp16 weights stand 2^LIFT higher, between 2^7 and 2^15 for a row's largest: what fp16 (at most 65504) has no number for
+    // begins at 2^-25, so beside a weight of 1 it would drop all below 2^-25 from the products and not from the sum (up to n_k 2^-25 of the largest value: 1e-3 at
+    // 32768 keys), and so only what is below 2^-32.  Sums and accumulators are as much larger, and every join takes them relative to their m.
     __device__ __forceinline__ void follow(int i, float mx) {
-        if (__builtin_expect_with_probability(__builtin_amdgcn_ballot_w64(mx > m[i] + 8.f) != 0, 0, 0.999)) {
-            const float m_new = fmaxf(m[i], mx), alpha = __builtin_amdgcn_exp2f(m[i] - m_new);
+        if (__builtin_expect_with_probability(__builtin_amdgcn_ballot_w64(mx > m[i] + (8.f + LIFT)) != 0, 0, 0.999)) {
+            const float m_new = fmaxf(m[i], mx - LIFT), alpha = __builtin_amdgcn_exp2f(m[i] - m_new);
             m[i] = m_new;
             l[i] *= alpha;
 #pragma unroll

@@ -82,3 +82,49 @@ def test_gelu_rows_far_out(ops):
         got = ops.gelu_(x.clone())
         bound = 2e-6 + (u(t) + U32) * torch.nan_to_num(want.abs(), nan=0.0, posinf=0.0) + tiny(t)
         within(f"gelu rows {t}", got, torch.where(nan, xd, want), bound)
+
+
+# ----------------------------------------------------------------------------------------------------------- attn_diff
+# wave form with one share, with shares and a join, one workgroup, many rows
+ATTN_FORMS = [(600, 1, 4, 2, 300), (1, 1, 8, 8, 4099), (2, 3, 8, 2, 250), (16, 200, 4, 4, 1000)]
+
+
+def heads_of(t, B, n, H):
+    """[128] channel values in every row of [B, n, H, 128]."""
+    return t.to("cuda")[None, None, None].expand(B, n, H, 128).contiguous()
+
+
+@pytest.mark.parametrize("B,n_q,H,KV,n_k", ATTN_FORMS)
+@pytest.mark.parametrize("norm", [False, True], ids=["plain", "norm"])
+def test_attn_small_weights_beside_a_large_one(ops, B, n_q, H, KV, n_k, norm):
+    """fp16: one key of value 0 takes almost everything, the other keys' weights are 2^-26 of it, and they alone make the result.
+    A weight stands at least 2^7 times as high as relative to the row's largest, so it is rounded by u, or below fp16's normals by 2^-25 / 2^7: each map is off by at most
+    (u + d) A|V| + n_k 2^-32 max|V|, d as in test_gpu_block_ops.attn64; A's own difference follows."""
+    randn = gen(960)
+    step = torch.full((128,), 1.0)
+    q = heads_of(step, B, n_q, H).to(F16)
+    k = randn(B, n_k, KV, 128, scale=0.02).to(F16)
+    k[:, 0] = 2.25          # 64 * 2.25 / 8 = 18, and 18 log2(e) = 25.97
+    v = (64 + randn(B, n_k, KV, 128, scale=8.0)).to(F16)
+    v[:, 0] = 0
+    lam, lam_init = torch.zeros(4, 64, device="cuda"), 0.4
+    gamma = 1 + randn(128, scale=0.1) if norm else None
+    got = ops.attn_diff(q, k, v, lam, lam_init, gamma=gamma, eps=1e-12)
+    want, bound = torch.zeros(B, n_q, H, 128, dtype=torch.float64, device="cuda"), None
+    bound = torch.zeros_like(want)
+    d = 70 * U32 * 64 * 2.25 / 8 + 8 * U32 + (n_k / 32 + 8) * U32 * 2
+    for h in range(H):
+        kh = h // (H // KV)
+        o, b = 0.0, 0.0
+        for i, f in ((0, 1.0), (1, -lam_init)):
+            s = q[:, :1, h, 64 * i:64 * i + 64].double() @ k[:, :, kh, 64 * i:64 * i + 64].double().transpose(1, 2).contiguous() / 8          # all queries are the same
+            a = torch.softmax(s, -1)
+            o = o + f * (a @ v[:, :, kh].double())
+            b = b + abs(f) * ((u(F16) + 2 * d) * (a @ v[:, :, kh].double().abs()) + n_k * 2.0 ** -32 * v[:, :, kh].double().abs().max().item())
+        if norm:
+            rms = (o.square().mean(-1, keepdim=True) + 1e-12).sqrt()
+            g = gamma.double().abs() * (1 - lam_init)
+            b = g / rms * (b + o.abs() / rms * b.square().mean(-1, keepdim=True).sqrt())
+            o = o * gamma.double() * (1 - lam_init) / rms
+        want[:, :, h], bound[:, :, h] = o, b + (u(F16) + 8 * U32) * (o.abs() + b) + tiny(F16)
+    within(f"attn small weights {B} {n_q}x{n_k} {H}/{KV}", got, want, bound)
