@@ -44,6 +44,10 @@ __device__ __forceinline__ float diff_norm(float square_sum, const DiffArgs& p) 
     return d == 0.f ? 0.f : (1.f - p.lambda_init) / sqrtf(d);
 }
 
+// `num` over a map's sum of weights.  A sum of 0 is that of a query that sees no key, whose result is zeros -- or of one whose scores are all -inf: they
+// have no softmax, and the result is NaN.  (The largest finite score has a weight of 1 or more.)
+__device__ __forceinline__ float diff_over(float num, float sum, int seen) { return sum == 0.f ? (seen > 0 ? NAN : 0.f) : num / sum; }
+
 // keys of sequence b, in [0, n_k] whatever the lengths' tensor holds
 __device__ __forceinline__ int key_count(const DiffArgs& p, int b) { return p.k_len ? max(0, min(p.k_len[b], p.n_k)) : p.n_k; }
 // number of keys query q sees
@@ -287,7 +291,7 @@ template <class E, bool Q_LDS = false> struct DiffWave {
     // swizzled by the row) and leave as whole rows, four to an instruction.
     __device__ __forceinline__ void finish(const DiffArgs& p, int b, int h, int row0, int rows, uint32_t buf, int lane, float lam) {
         join_halves();
-        const float w0 = l[0] == 0.f ? 0.f : 1.f / l[0], w1 = l[1] == 0.f ? 0.f : lam / l[1];
+        const float w0 = diff_over(1.f, l[0], seen), w1 = diff_over(lam, l[1], seen);
         float ss = 0.f;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -519,7 +523,9 @@ template <class E> struct Joined {
     }
     // lam: diff_lambda, g: the lane's two channels of gamma, both requested before the wait for the shares
     __device__ __forceinline__ void finish(const DiffArgs& p, int b, int h, int row, int lane, float lam, float2 g) const {
-        const float w0 = l[0] == 0.f ? 0.f : 1.f / l[0], w1 = l[1] == 0.f ? 0.f : lam / l[1];
+        int seen = 0;
+        if (l[0] == 0.f || l[1] == 0.f) seen = seen_by(p, b, key_count(p, b), row / p.group);
+        const float w0 = diff_over(1.f, l[0], seen), w1 = diff_over(lam, l[1], seen);
         float y0 = o[0][0] * w0 - o[1][0] * w1, y1 = o[0][1] * w0 - o[1][1] * w1;
         if (p.gamma) {
             const float norm = diff_norm(wave_sum(fmaf(y0, y0, y1 * y1)), p);

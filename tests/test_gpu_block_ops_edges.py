@@ -128,3 +128,20 @@ def test_attn_small_weights_beside_a_large_one(ops, B, n_q, H, KV, n_k, norm):
             o = o * gamma.double() * (1 - lam_init) / rms
         want[:, :, h], bound[:, :, h] = o, b + (u(F16) + 8 * U32) * (o.abs() + b) + tiny(F16)
     within(f"attn small weights {B} {n_q}x{n_k} {H}/{KV}", got, want, bound)
+
+
+@pytest.mark.parametrize("t", [F16, BF16], ids=str)
+@pytest.mark.parametrize("B,n_q,H,KV,n_k", ATTN_FORMS)
+def test_attn_scores_of_minus_infinity_are_not_an_empty_row(ops, t, B, n_q, H, KV, n_k):
+    """Every score of the rows that see a key is -inf (an infinity in each key): no softmax exists, the result is NaN, as for any infinity; a row that sees no key is zeros."""
+    randn = gen(970)
+    q, k, v = randn(B, n_q, H, 128).to(t), randn(B, n_k, KV, 128).to(t), randn(B, n_k, KV, 128).to(t)
+    q[..., 0], q[..., 64] = 1.0, 1.0
+    for at in (0, 64):          # in one map, then in the other
+        k2 = k.clone()
+        k2[..., at] = float("-inf")
+        lens = torch.full((B,), n_k, dtype=torch.int32, device="cuda")
+        lens[-1] = 0 if B > 1 else n_k
+        got = ops.attn_diff(q, k2, v, torch.zeros(4, 64, device="cuda"), 0.4, k_len=lens)
+        assert torch.isnan(got[:B - (B > 1)]).all()
+        assert B == 1 or got[-1].eq(0).all()
