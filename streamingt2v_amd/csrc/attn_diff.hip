@@ -39,8 +39,8 @@ __device__ __forceinline__ float diff_lambda(const float* lam, float lambda_init
 }
 
 // the factor of the head's norm; zeros stay zeros with eps = 0 too
-__device__ __forceinline__ float diff_norm(float square_sum, const DiffArgs& p) {
-    const float d = square_sum * (1.f / 128.f) + p.eps;
+__device__ __forceinline__ float diff_norm(float square_sum, const DiffArgs& p, float eps) {
+    const float d = square_sum * (1.f / 128.f) + eps;
     return d == 0.f ? 0.f : (1.f - p.lambda_init) / sqrtf(d);
 }
 
@@ -301,7 +301,19 @@ template <class E, bool Q_LDS = false> struct DiffWave {
                 ss = fmaf(o[0][t][r], o[0][t][r], ss);
             }
         ss += __shfl_xor(ss, 32, 64);
-        const float norm = p.gamma ? diff_norm(ss, p) : 1.f;
+        const float f = p.gamma ? svd_rms_factor(ss, p.eps) : 1.f;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(f != 1.f) != 0, 0)) {          // (others' values times 1, the same sum again)
+            ss = 0.f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    o[0][t][r] *= f;
+                    ss = fmaf(o[0][t][r], o[0][t][r], ss);
+                }
+            ss += __shfl_xor(ss, 32, 64);
+        }
+        const float norm = p.gamma ? diff_norm(ss, p, p.eps * f * f) : 1.f;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -528,7 +540,13 @@ template <class E> struct Joined {
         const float w0 = diff_over(1.f, l[0], seen), w1 = diff_over(lam, l[1], seen);
         float y0 = o[0][0] * w0 - o[1][0] * w1, y1 = o[0][1] * w0 - o[1][1] * w1;
         if (p.gamma) {
-            const float norm = diff_norm(wave_sum(fmaf(y0, y0, y1 * y1)), p);
+            float ss = wave_sum(fmaf(y0, y0, y1 * y1));
+            const float f = svd_rms_factor(ss, p.eps);          // the same in all lanes
+            if (f != 1.f) {
+                y0 *= f; y1 *= f;
+                ss = wave_sum(fmaf(y0, y0, y1 * y1));
+            }
+            const float norm = diff_norm(ss, p, p.eps * f * f);
             y0 *= norm * g.x; y1 *= norm * g.y;
         }
         *(uint32_t*)(p.O + b * p.o_sb + (row / p.group) * p.o_st + (h * p.group + row % p.group) * p.o_sh + 2 * lane) = E::pack(y0, y1);

@@ -145,3 +145,16 @@ def test_attn_scores_of_minus_infinity_are_not_an_empty_row(ops, t, B, n_q, H, K
         got = ops.attn_diff(q, k2, v, torch.zeros(4, 64, device="cuda"), 0.4, k_len=lens)
         assert torch.isnan(got[:B - (B > 1)]).all()
         assert B == 1 or got[-1].eq(0).all()
+
+
+@pytest.mark.parametrize("B,n_q,H,KV,n_k", ATTN_FORMS)
+def test_attn_head_norm_of_values_whose_squares_leave_fp32(ops, B, n_q, H, KV, n_k):
+    """bf16 values of 1e-30 (with eps = 0) to 1e30: the head's norm is the formula's.  With eps = 0 the result of values times 2^c is that of the values:
+    the products and sums scale exactly, and the norm's factor is rounded anew (8 U32) in front of the result's rounding (both results': 2 u)."""
+    randn = gen(980)
+    q, k, v = randn(B, n_q, H, 128).to(BF16), randn(B, n_k, KV, 128).to(BF16), randn(B, n_k, KV, 128).to(BF16)
+    lam, gamma = randn(4, 64, scale=0.1), 1 + randn(128, scale=0.1)
+    want = ops.attn_diff(q, k, v, lam, 0.4, gamma=gamma, eps=0.0)
+    for c in (-90, -70, 70, 100):
+        got = ops.attn_diff(q, k, (v.float() * 2.0 ** c).to(BF16), lam, 0.4, gamma=gamma, eps=0.0)
+        within(f"attn head norm 2^{c} {B} {n_q}x{n_k}", got, want, (u(BF16) * 2 + 8 * U32) * want.double().abs() + tiny(BF16))
