@@ -702,7 +702,8 @@ extern "C" int svd_attn_diff(const svd_bf16* Q, int64_t q_sb, int64_t q_st, int6
     const DiffArgs p = {Q, q_sb, q_st, q_sh, K, k_sb, k_st, k_sh, V, v_sb, v_st, v_sh, O, o_sb, o_st, o_sh, lam, lambda_init, gamma, eps, k_len, q_start,
                         n_q, n_k, kv_heads, group, causal};
     const int64_t grid = (int64_t)plan.row_blocks * batch * kv_heads * plan.shares;
-    if (grid > 0x7fffffff || (int64_t)batch * heads * n_q > 0x7fffffff) return SVD_EINVAL;
+    const int threads = plan.form == ROWS ? 256 : plan.form == GROUP ? GROUP_WAVES * 64 : 64;
+    if (grid > 0xffffffff / threads || (int64_t)batch * heads * n_q > 0x7fffffff) return SVD_EINVAL;          // (a launch has less than 2^32 threads)
     if (plan.form == ROWS) {
         constexpr int LDS = 8 * 32 * ROW_B + 4 * Q_B;          // rings and map 2's queries: 76 KiB, two workgroups on a CU (two of 80 do not fit)
         SVD_DISPATCH_DTYPE(dtype, {
