@@ -955,6 +955,21 @@ def _vec(t, n):
     return t is None or (t.dtype == torch.float32 and t.shape == (n,) and (n == 1 or t.stride(0) == 1))
 
 
+def _apart(out, *inputs):
+    """Does the 2-D out share no byte with the 2-D inputs?  (Column ranges of the same rows may lie between each other.)"""
+    for t in inputs:
+        if out.numel() == 0 or t.numel() == 0 or out.untyped_storage().data_ptr() != t.untyped_storage().data_ptr():
+            continue
+        a, b, la, lb = out.data_ptr(), t.data_ptr(), _ld(out) * out.element_size(), _ld(t) * t.element_size()
+        wa, wb = out.shape[1] * out.element_size(), t.shape[1] * t.element_size()
+        if a + (out.shape[0] - 1) * la + wa <= b or b + (t.shape[0] - 1) * lb + wb <= a:
+            continue
+        if out.shape[0] > 1 and t.shape[0] > 1 and la == lb > 0 and wa <= (b - a) % la <= la - wb:
+            continue
+        return False
+    return True
+
+
 def rmsnorm(x, gamma=None, *, eps=1e-6, residual=None, f8=False, out=None, out_sum=None):
     """s = x (+ residual); y = s * gamma / sqrt(mean(s^2) + eps) per row.
 
@@ -1000,7 +1015,7 @@ def linear_act(x, w, *, bias=None, act=None, residual=None, x_scale=None, w_scal
     x [M, K], w [N, K]: both fp16, both bf16, or both e4m3 (x_scale [M], w_scale [N] fp32 or None, e.g. from rmsnorm(f8=True)); bias [N] fp32;
     act: None | "relu" | "gelu" (erf) | "gelu_tanh" | "silu"; residual [M, N] of the 16-bit type or fp32, added AFTER the activation.
     The result is of out_dtype: the 16-bit type (for e4m3 operands: ops.ELEM, or the one named) or fp32.  out: a destination with contiguous columns; it may be
-    the residual itself."""
+    the residual itself, but shares no memory with x and w."""
     dev = _on(x, w, bias, residual, x_scale, w_scale, out)
     assert x.dim() == 2 and w.dim() == 2 and x.shape[1] == w.shape[1] and x.dtype == w.dtype and act in _l.ACT
     M, K = x.shape
@@ -1019,6 +1034,7 @@ def linear_act(x, w, *, bias=None, act=None, residual=None, x_scale=None, w_scal
     assert _vec(bias, N) and _vec(x_scale, M) and _vec(w_scale, N)
     assert residual is None or (residual.shape == (M, N) and residual.dtype in (e, torch.float32))
     assert out is None or (out.shape == (M, N) and out.dtype == out_dtype)
+    assert out is None or _apart(out, x, w), "out shares memory with x or w"
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return linear_act(x, w, bias=bias, act=act, residual=residual, x_scale=x_scale, w_scale=w_scale, out_dtype=out_dtype, out=out)
@@ -1061,7 +1077,7 @@ def attn_diff(q, k, v, lam, lambda_init, *, gamma=None, eps=1e-5, causal=False, 
     ranges of a projection's rows, a cache, (frame, pixel) rows transposed); lam [4, 64] fp32: lq1, lk1, lq2, lk2.
     k_len [batch] int32: keys of each sequence (rows behind them are not read).  causal: query i of sequence b stands at position q_start[b] + i (int32
     [batch]; None: the last query stands at the last key) and sees the keys up to there.  A query that sees no key gives zeros.
-    Returns [batch, n_q, heads, 128] (out, if given)."""
+    Returns [batch, n_q, heads, 128] (out, if given; it may be q itself, but shares no memory with k and v)."""
     dev = _on(q, k, v, lam, gamma, k_len, q_start, out)
     assert q.dim() == 4 and k.dim() == 4 and q.shape[3] == 128 and k.shape == v.shape and k.shape[3] == 128 and k.shape[0] == q.shape[0]
     assert q.dtype in _SIXTEEN and k.dtype == q.dtype and v.dtype == q.dtype
@@ -1073,6 +1089,7 @@ def attn_diff(q, k, v, lam, lambda_init, *, gamma=None, eps=1e-5, causal=False, 
     assert k_len is None or (k_len.dtype == torch.int32 and k_len.shape == (B,) and k_len.is_contiguous())
     assert q_start is None or (causal and q_start.dtype == torch.int32 and q_start.shape == (B,) and q_start.is_contiguous())
     assert out is None or (out.shape == q.shape and out.dtype == q.dtype)
+    assert out is None or out.numel() == 0 or (out.data_ptr() != k.data_ptr() and out.data_ptr() != v.data_ptr()), "out is k or v"
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return attn_diff(q, k, v, lam, lambda_init, gamma=gamma, eps=eps, causal=causal, k_len=k_len, q_start=q_start, out=out)
