@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_block_ops import BF16, F16, F32, F8, U32, check_norm, gen, ops, tiny, u, within  # noqa: F401
+from tests.test_gpu_block_ops import ACTS, BF16, F16, F32, F8, U32, check_linear, check_norm, gen, make_linear, ops, run_attn, tiny, u, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -48,6 +48,18 @@ def test_rmsnorm_rows_whose_squares_leave_fp32(ops, eps, f8):
             check_norm(f"rmsnorm squares out of range {ch} {xt} {rt}", ops.rmsnorm(x, gamma, eps=eps, residual=r, f8=f8), x, r, gamma, eps, f8)
 
 
+@pytest.mark.parametrize("f8", [False, True], ids=["e16", "e4m3"])
+def test_rmsnorm_fp32_rows_with_a_16_bit_residual(ops, f8):
+    """fp32 x on a residual of the package's 16-bit type: the sum goes on in 16 bits, in place too."""
+    for i, ch in enumerate(NORM_WIDTHS):
+        randn = gen(930 + i)
+        x, r = randn(7, ch), randn(7, ch, scale=3.0).to(ops.ELEM)
+        gamma = 1 + randn(ch, scale=0.1) if i % 2 else None
+        check_norm(f"rmsnorm fp32 + 16 bit {ch}", ops.rmsnorm(x, gamma, residual=r, f8=f8), x, r, gamma, 1e-6, f8)
+        before = r.clone()
+        check_norm(f"rmsnorm fp32 + 16 bit {ch} in place", ops.rmsnorm(x, gamma, residual=r, out_sum=r, f8=f8), x, before, gamma, 1e-6, f8)
+
+
 # ---------------------------------------------------------------------------------------------------------- linear_act
 FAR = [0.0, -0.0, 1e-30, -1e-30, 1.0, -1.0, 6.99, -6.99, 7.0, -7.0, 7.01, -7.01, 50.0, -50.0, 1e4, -1e4, 1e7, -1e7, 1e9, -1e9, 1e12, -1e12, 1e30, -1e30, 3e38, -3e38]
 
@@ -82,6 +94,39 @@ def test_gelu_rows_far_out(ops):
         got = ops.gelu_(x.clone())
         bound = 2e-6 + (u(t) + U32) * torch.nan_to_num(want.abs(), nan=0.0, posinf=0.0) + tiny(t)
         within(f"gelu rows {t}", got, torch.where(nan, xd, want), bound)
+
+
+@pytest.mark.parametrize("act", [None, "relu", "silu", "gelu_tanh"])
+@pytest.mark.parametrize("m,n,k", [(1, 300, 64), (300, 1041, 128), (1100, 1040, 2064), (4400, 2100, 64)])
+def test_linear_activations_far_out(ops, act, m, n, k):
+    """As for gelu: the other activations from the bias alone, to both ends of fp32, the infinities and NaN: 2e-6, and four roundings of a large result."""
+    x, w = torch.zeros(m, k, device="cuda").to(BF16), gen(941)(n, k).to(BF16)
+    bias = torch.tensor(FAR, device="cuda").repeat(-(-n // len(FAR)))[:n].contiguous()
+    bias[n - 1], bias[n // 2], bias[n // 3] = float("inf"), float("-inf"), float("nan")
+    want = ACTS[act](bias.double())
+    for od in (F32, BF16):
+        got = ops.linear_act(x, w, bias=bias, act=act, out_dtype=od)
+        within(f"{act} far out {m}x{n}x{k} {od}", got[-1], want, 2e-6 + (u(od) + 4 * U32) * torch.nan_to_num(want.abs(), nan=0.0, posinf=0.0) + tiny(od))
+
+
+@pytest.mark.parametrize("t", [BF16, F8], ids=str)
+def test_linear_far_rows(ops, t):
+    """Rows 2^23 bytes and more apart (tiles copy them), and rows of more than 2^23 bytes (few of them)."""
+    es = 1 if t == F8 else 2
+    ld = (1 << 23) // es + 16
+    randn, x, w, sx, sw = make_linear(880, 1100, 1040, 320, t)
+    far = torch.zeros(1100, ld * es, dtype=torch.uint8, device="cuda").view(t)[:, 8:328]
+    far.view(torch.uint8).copy_(x.view(torch.uint8))
+    check_linear("linear far rows", ops.linear_act(far, w, x_scale=sx, w_scale=sw, act="silu", out_dtype=BF16), x, w, sx, sw, None, "silu", None)
+    del far
+    k = (1 << 23) // es + 37
+    randn, x, w, sx, sw = make_linear(881, 3, 5, k, t)
+    got = ops.linear_act(x, w, x_scale=sx, w_scale=sw, out_dtype=F32)
+    scale = sx.double()[:, None] * sw.double()[None] if sx is not None else 1.0
+    # all ones in front of it: whole numbers below 2^24 are exact, so a piece of K that is left out or counted twice shows as another number
+    one = torch.ones(3, k, device="cuda").to(t)
+    assert ops.linear_act(one, one[:2], out_dtype=F32).eq(k).all()
+    within("linear long rows", got, (x.double() @ w.double().t()) * scale, (k + 8) * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t()) * scale)
 
 
 # ----------------------------------------------------------------------------------------------------------- attn_diff
@@ -158,3 +203,20 @@ def test_attn_head_norm_of_values_whose_squares_leave_fp32(ops, B, n_q, H, KV, n
     for c in (-90, -70, 70, 100):
         got = ops.attn_diff(q, k, (v.float() * 2.0 ** c).to(BF16), lam, 0.4, gamma=gamma, eps=0.0)
         within(f"attn head norm 2^{c} {B} {n_q}x{n_k}", got, want, (u(BF16) * 2 + 8 * U32) * want.double().abs() + tiny(BF16))
+
+
+@pytest.mark.parametrize("t", [F16, BF16], ids=str)
+@pytest.mark.parametrize("B,n_q,H,KV,n_k", [(600, 1, 4, 2, 100), (2, 1, 8, 4, 3000), (3, 4, 8, 2, 200), (40, 200, 4, 4, 300)])
+def test_attn_shared_prefix_views(ops, t, B, n_q, H, KV, n_k):
+    """One cache for the whole batch (a batch stride of 0), one head's keys for every head (a head stride of 0), the same queries for every sequence; queries updated in place."""
+    randn = gen(990)
+    k, v = randn(1, n_k, KV, 128).to(t).expand(B, n_k, KV, 128), randn(1, n_k, 1, 128).to(t).expand(B, n_k, KV, 128)
+    q = randn(1, n_q, H, 128).to(t).expand(B, n_q, H, 128)
+    got = run_attn(ops, "attn shared prefix", q, k, v, 1, causal=n_q > 1)
+    assert torch.equal(got, got[:1].expand_as(got).contiguous())
+    q = randn(B, n_q, H, 128).to(t)
+    want = run_attn(ops, "attn shared prefix, queries of their own", q, k, v, 2, causal=n_q > 1)
+    randn = gen(5002)
+    lam, lam_init = randn(4, 64, scale=0.1), 0.8 - 0.6 * math.exp(-0.6)
+    got = ops.attn_diff(q, k, v, lam, lam_init, gamma=1 + randn(128, scale=0.1), causal=n_q > 1, out=q)
+    assert got.data_ptr() == q.data_ptr() and torch.equal(q, want), "in place of the queries"
