@@ -300,6 +300,15 @@ template <class E, bool Q_LDS = false> struct DiffWave {
                 o[0][t][r] = o[0][t][r] * w0 - o[1][t][r] * w1;
                 ss = fmaf(o[0][t][r], o[0][t][r], ss);
             }
+        // gamma is requested here, in front of the branch: behind it every piece would wait for its own (25 frames: 176 us, 128 like this)
+        float g[64];
+        if (p.gamma) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e) g[e] = p.gamma[8 * (e >> 2) + 4 * hi + (e & 3)];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 64; ++e) g[e] = 1.f;
+        }
         ss += __shfl_xor(ss, 32, 64);
         const float f = p.gamma ? svd_rms_factor(ss, p.eps) : 1.f;
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(f != 1.f) != 0, 0)) {          // (others' values times 1, the same sum again)
@@ -321,7 +330,7 @@ template <class E, bool Q_LDS = false> struct DiffWave {
                 const int d = 32 * t + 2 * r + 4 * hi;
                 float y[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = o[0][t][r + j] * (p.gamma ? norm * p.gamma[d + j] : 1.f);
+                for (int j = 0; j < 4; ++j) y[j] = o[0][t][r + j] * (norm * g[16 * t + r + j]);
                 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
                 const u32x2_t v = {E::pack(y[0], y[1]), E::pack(y[2], y[3])};
                 *(__attribute__((address_space(3))) u32x2_t*)(buf + l31 * ROW_B + (((d >> 3) ^ (l31 & 15)) << 4) + (d & 4) * 2) = v;
@@ -344,7 +353,7 @@ template <class E, bool Q_LDS = false> struct DiffWave {
 // matrix unit (24 instructions of 32 cycles), so the two have to run at once inside a wave.  The maps take turns: while map 1's weights of step j are made, the matrix unit
 // does map 2's scores of step j and its products with V of step j - 1; while map 2's weights are made, map 1's scores of step j + 1 and its products with V of step j.
 // So K is read a step ahead and V a step behind: rings of four 8-KiB slots each, requests two steps ahead, one barrier a step.
-// 2 x 9216 tokens, 5 heads, fp16: 782 us (0.83 PFLOP/s of the one-pass work, 0.97 with the rests' products; the clock falls to 1.9 GHz under it; 720 workgroups on 512
+// 2 x 9216 tokens, 5 heads, fp16: 780 us (0.84 PFLOP/s of the one-pass work, 0.97 with the rests' products; the clock falls to 1.9 GHz under it; 720 workgroups on 512
 // places leave the second round half empty).  Before the maps took turns: 828 us without the rests.  4 causal prompts of 1001 to 2001 tokens, 8 heads on 4: 81 us (104
 // with long rows first everywhere).
 template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kernel(DiffArgs p, int row_blocks) {
@@ -447,7 +456,7 @@ template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kern
 }
 
 // Few queries: one wave per (sequence, key / value head, 32 rows, share of the keys), no workgroup barrier; tiles of 32 keys, two in turn.  With one share
-// the wave finishes the rows (2304 x 10 heads of 25 frames: 173 us, 3.4 TB/s; 16 KiB requested by each of 8 waves a CU); else it leaves maxima, sums and both accumulators in the scratch memory (fp32, [row][share][260]) for the join
+// the wave finishes the rows (2304 x 10 heads of 25 frames: 128 us, 4.6 TB/s; 16 KiB requested by each of 8 waves a CU); else it leaves maxima, sums and both accumulators in the scratch memory (fp32, [row][share][260]) for the join
 // (8 caches of 16 to 32 k keys, 16 heads on 4: 90 us, 4.7 TB/s, and 5 for the join; one of 1025 keys, 8 heads: 6 and 3).
 template <class E> __global__ __launch_bounds__(64, 2) void attn_diff_wave_kernel(DiffArgs p, int row_blocks, int shares, float* ws) {
     constexpr int KT = 32, TILE_B = KT * ROW_B, BUF_B = 2 * TILE_B;
