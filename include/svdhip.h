@@ -417,7 +417,8 @@ int svd_linear_act(const void* X, int64_t ldx, const void* W, int64_t ldw, const
  *   lam [4][64] fp32: lq1, lk1, lq2, lk2.   gamma [128] fp32 or NULL (then eps is not used and nothing is scaled by 1 - lambda_init).
  *   k_len [batch] or NULL: keys of each sequence (clamped to 0..n_k; NULL: n_k); rows of K and V behind them are not read.
  *   causal: query i stands at position q_start[b] + i (q_start NULL: the last query stands at the last key) and sees keys up to and including its position.
- *   A query that sees no key gives zeros; values at positions that it does not see never reach it, NaN and Inf included.
+ *   A query that sees no key gives zeros (one whose scores are all -inf: NaN); values at positions that it does not see never reach it, NaN and Inf included.  Products are summed
+ *   before they are divided by the weights' sum, at up to 2^8 times their size (fp16: 2^15): bf16 values of more than 2^120 / n_k may overflow.  O may be Q; it shares no memory with K and V.
  *   ws: svd_attn_diff_ws_bytes(...) bytes of scratch memory (16-byte aligned; may be NULL when that is 0), free again when the call's work on `stream` ends. */
 int64_t svd_attn_diff_ws_bytes(int32_t batch, int32_t n_q, int32_t n_k, int32_t heads, int32_t kv_heads);
 int svd_attn_diff(const svd_bf16* Q, int64_t q_sb, int64_t q_st, int64_t q_sh, const svd_bf16* K, int64_t k_sb, int64_t k_st, int64_t k_sh,

@@ -354,7 +354,7 @@ template <class E, bool Q_LDS = false> struct DiffWave {
 // does map 2's scores of step j and its products with V of step j - 1; while map 2's weights are made, map 1's scores of step j + 1 and its products with V of step j.
 // So K is read a step ahead and V a step behind: rings of four 8-KiB slots each, requests two steps ahead, one barrier a step.
 // 2 x 9216 tokens, 5 heads, fp16: 780 us (0.84 PFLOP/s of the one-pass work, 0.97 with the rests' products; the clock falls to 1.9 GHz under it; 720 workgroups on 512
-// places leave the second round half empty).  Before the maps took turns: 828 us without the rests.  4 causal prompts of 1001 to 2001 tokens, 8 heads on 4: 81 us (104
+// places leave the second round half empty).  Before the maps took turns: 828 us without the rests.  4 causal prompts of 1001 to 2001 tokens, 8 heads on 4: 80 us (104
 // with long rows first everywhere).
 template <class E> __global__ __launch_bounds__(256, 2) void attn_diff_rows_kernel(DiffArgs p, int row_blocks) {
     constexpr int SLOT_B = 32 * ROW_B, RING_B = 4 * SLOT_B;          // K ring, then V ring
@@ -600,7 +600,7 @@ template <class E> __global__ __launch_bounds__(256) void attn_diff_join_kernel(
 }
 
 // A few rows and at most 256 keys: one workgroup per (sequence, key / value head), 32 keys to each of its eight waves, joined in LDS: one launch and no scratch memory.
-// 8 heads, 100 / 256 keys: 6.8 / 7.7 us in a graph, 11.3 called one by one; shares and join 9.7 / 9.1 and 15.5.  (More keys, as a loop over tiles: 513 keys 11.6 against 9.7 us.)
+// 8 heads, 100 / 256 keys: 6.4 / 7.8 us in a graph, 11.3 called one by one; shares and join 9.7 / 9.1 and 15.5.  It takes all 256 registers and spills 14 (60 bytes a lane).  (More keys, as a loop over tiles: 513 keys 11.6 against 9.7 us.)
 constexpr int GROUP_WAVES = 8, GROUP_ROWS = 16, GROUP_KEYS = GROUP_WAVES * 32, GROUP_LDS = GROUP_WAVES * (64 * ROW_B + GROUP_ROWS * 16);
 template <class E> __global__ __launch_bounds__(GROUP_WAVES * 64, 2) void attn_diff_group_kernel(DiffArgs p) {
     constexpr int TILE_B = 32 * ROW_B;
@@ -665,7 +665,13 @@ template <class E> __global__ __launch_bounds__(GROUP_WAVES * 64, 2) void attn_d
     }
 }
 
-// Which form: see svd_attn_diff
+// Which form.  Both sides measured, us a call in a graph, fp16, 128 channels, all keys | causal:
+//   many rows (128 to a workgroup, keys staged once for four waves) with more than 64 rows and 128 blocks of 128, else waves of 32 rows with the keys in shares: with fewer rows half
+//     of a block's waves have none, with fewer blocks half of the CUs have none, and shares fill them.
+//     64 rows, 2048 keys, 128 blocks (16 x 64 tokens, 8 heads): many-row form 67.6 | 69.7, waves 62.6 | 62.8; 65 rows: 68.1 | 70.7, 99.9 | 101; 128 rows 71.7 | 74.2, 106 | 106.
+//     1 x 2000 tokens: 4 heads (64 blocks) 67.6 | 69.5, 67.8 | 50.3; 6 (96) 69.7 | 69.8, 95.8 | 67.2; 8 (128) 68.4 | 69.7, 107 | 79.5; 1 x 4096 tokens: 2 heads (64) 128 | 132, 84.0 | 70.7;
+//     4 (128) 129 | 133, 148 | 128.  With few keys the border lies lower than the rule has it: 4 x 300 tokens, 8 heads (96 blocks) 17.7 | 19.8, 40.3 | 33.7.
+//   one workgroup for up to 16 rows on up to 256 keys: see attn_diff_group_kernel.
 enum { ROWS, WAVES, GROUP };
 struct Plan { int form, row_blocks, shares; int64_t ws; };
 Plan plan_for(int64_t batch, int64_t n_q, int64_t n_k, int64_t heads, int64_t kv_heads) {
@@ -725,7 +731,7 @@ extern "C" int svd_attn_diff(const svd_bf16* Q, int64_t q_sb, int64_t q_st, int6
             hipLaunchKernelGGL((attn_diff_group_kernel<E>), dim3((unsigned)grid), dim3(GROUP_WAVES * 64), GROUP_LDS, (hipStream_t)stream, p);
         });
     } else {
-        const int LDS = (n_k > 32 ? 4 : 2) * 32 * ROW_B;          // one tile needs no second buffer: 8 waves on a CU instead of 5 (25 keys x 23040 heads: 173 us, 300 with two and rows written 8 bytes at a time)
+        const int LDS = (n_k > 32 ? 4 : 2) * 32 * ROW_B;          // one tile needs no second buffer: 8 waves on a CU instead of 5 (25 keys x 23040 heads: 128 us; 174 when it was measured, 300 with two and rows written 8 bytes at a time)
         SVD_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((attn_diff_wave_kernel<E>), dim3((unsigned)grid), dim3(64), LDS, (hipStream_t)stream, p, plan.row_blocks, plan.shares, (float*)ws));
         SVD_CHECK_LAUNCH("attn_diff");
         if (plan.shares > 1)

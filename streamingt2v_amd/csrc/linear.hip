@@ -113,9 +113,11 @@ template <int EB> __device__ __forceinline__ uint4 load_chunk(const char* row, i
 // step after the next: two halves of a step (2000 cycles of matrix work) ahead of its use, one barrier a step.
 // W's rows lie in LDS as even, then odd columns of each 64: a lane's two tiles of such a block are two adjacent columns, so results leave (and residuals come) as
 // pairs, 32 lanes a contiguous 128 (fp32: 256) bytes of a row.
-// Measured, 256 x 256: bf16 28800 x 1280 x 5120 onto an fp32 stream 392 us (0.96 PFLOP/s; two whole rounds 320 us, the split third 43, the join 17), e4m3
-// 28800 x 5120 x 1280 with GELU 264 us (1.43 PFLOP/s).  The same loop without its requests and LDS reads takes 232 of the 320 us (1.47 PFLOP/s, what a large library
-// product reaches), without either of them 286; of the 264 us the epilogue is about 90: one workgroup fills a CU, so nothing runs beside it.
+// Measured, 256 x 256: bf16 28800 x 1280 x 5120 onto an fp32 stream 390 us (0.97 PFLOP/s; two whole rounds 320 us, the split third 43, the join 17), e4m3
+// 28800 x 5120 x 1280 with GELU 260 us (1.45 PFLOP/s), 226 without scales, bias and activation; e4m3 to fp32 (widened, 128 x 128) 374.  The same loop without its requests and LDS
+// reads takes 232 of the 320 us (1.47 PFLOP/s, what a large library product reaches), without either of them 286; one workgroup fills a CU, so nothing runs beside its epilogue.
+// The whole-tile kernel takes all 256 registers and spills 32 (68 bytes a lane; 74 MB of the 369 that the e4m3 product writes); the kernel of the shares, the same loop
+// without the epilogue, 248 to 254 and none.
 template <int WM_, int WN_, int TM_, int TN_> struct Tile {
     static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, WAVES = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32, SLOT = (BM + BN) * 128, REQ = (BM + BN) / 8 / WAVES;
 };
@@ -462,7 +464,14 @@ using Small = Tile<2, 2, 2, 2>;            // 128 x 128, four waves, 64 KiB: two
 constexpr int CUS = 256;
 constexpr int ROWS_TWO = 256;
 
-// Which form, from sizes alone.
+// Which form, from sizes alone.  Both sides measured, us a call in a graph, bf16 | e4m3 to 16 bits:
+//   rows kernel below 64 tiles of 128 x 128, because such tiles leave most CUs without one, and shares of K cost a join:
+//     K = 1280, rows kernel against tiles: 20 tiles (256 x 1280) 10.8 | 7.5 against 12.9 | 9.9; 40 (512 x 1280) 18.0 | 10.8, 16.4 | 10.8; 60 (768 x 1280) 17.7 | 11.0, 17.1 | 12.1;
+//     64 (1024 x 1024) 17.7 | 11.0, 17.8 | 12.0; 70 (896 x 1280) 24.1 | 14.4, 18.6 | 12.5; 80 (1024 x 1280) 24.1 | 14.7, 19.1 | 13.1.
+//     With K = 5120 the border lies lower than the rule has it: 10 tiles (128 x 1280) 21.1 | 12.5, 16.7 | 14.3; 20 (256 x 1280) 33.5 | 17.2, 20.0 | 17.1; 60 (768 x 1280) 62.9 | 33.2, 25.4 | 25.5.
+//   256 x 256 from 128 of them on (a workgroup for every other CU), because they read half the operand bytes a product: K = 1280, 256 x 256 against 128 x 128:
+//     160 tiles (5120 x 2048) 36.0 | 24.9, 44.4 | 30.5; 300 (5120 x 3840) 72.0 | 47.9, 69.6 | 45.3; 2260 (28800 x 5120) e4m3 with GELU 260, 266; 565 (28800 x 1280 x 5120) bf16 390, 454.
+//     At 128 tiles (4096 x 2048) the rule begins too early: 41.1 | 34.0, 24.8 | 15.7, all of them split in two shares of K here and 512 places filled once there.
 enum { ROWS, BIG, SMALL };
 struct LinPlan { int form, whole, shares; int64_t ws; };
 template <class T> LinPlan rounds_of(int form, int64_t tm, int64_t tn, int64_t kbytes, int slots) {
