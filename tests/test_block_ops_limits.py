@@ -1,10 +1,9 @@
 """Refusals of svd_attn_diff and the block's launchers at the edge of what a call can hold (no GPU needed)."""
-import pytest  # noqa: F401
-
 import pytest
 import torch
 
 from tests.test_block_ops_args import EINVAL, _g, attn, f32, lib, nolaunch  # noqa: F401
+
 
 def test_attn_more_threads_than_a_launch_has(lib):
     """2^26 waves are 2^32 threads, which no launch has: refused like any other size, not handed to the driver."""
