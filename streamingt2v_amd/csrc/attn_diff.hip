@@ -8,7 +8,7 @@
 //                                      between the halves of the wave;
 //   O_i^T[channel][query] += V^T P_i^T  the accumulator registers 8 s .. 8 s + 7 of S_i^T are the B operand of step s as they stand, if the A operand holds
 //                                      the same keys in the same order: half h holds keys 16 s + 4 h + (0..3) and 16 s + 8 + 4 h + (0..3).
-// P is rounded to the 16-bit type for the matrix cores (at most half a step of the type relative to each weight, in fp16 at least 2^-32 of the row's largest); scores, maxima, sums and both accumulators
+// P is rounded to the 16-bit type for the matrix cores (at most half a step of the type relative to each weight, or in fp16 2^-32 of the row's largest); scores, maxima, sums and both accumulators
 // are fp32, and the row sums add the unrounded weights.  The maps' difference makes these roundings weigh more than the result's own (lambda 0.8, scores of
 // deviation 1: together 1.6 roundings of the result in the 2-norm), so what map 1's weights lose is rounded once more and multiplied as well: for all keys where the keys
 // and values are what takes the time (1.1 to 1.2 roundings), for 16 of 32 where the products are (1.45 at most; none, half, all of them: 727, 804, 896 us for 2 x 9216 tokens when it was measured).
